@@ -168,8 +168,7 @@ def prepare(case, seed):
 
     st = {"case": dict(case)}
     if case["op"] in ("bias", "attn"):
-        # a plane's table as the optimiser holds it, an attention layer's in the layer's type
-        st["table"] = rand(case["buckets"], case["heads"], dtype=torch.float32 if case["op"] == "bias" else dt)
+        st["table"] = rand(case["buckets"], case["heads"], dtype=torch.float32)
         both = case["both"] if case["op"] == "bias" else not case["causal"]
         st["map"] = torch.tensor(_map(case["buckets"], case["span"], both), dtype=torch.int32, device="cuda")
     if case["op"] == "bias":
@@ -296,7 +295,7 @@ def _run_attn(st):
         at = torch.arange(c["k_len"], device="cuda") - torch.arange(c["q_len"], device="cuda")[:, None] - shift[:, None, None]
         hide = hide | (at > 0)
     hide = hide[:, None]
-    s = q @ k.transpose(2, 3).contiguous() * scale + st["table"].float().t()[:, which].transpose(0, 1)
+    s = q @ k.transpose(2, 3).contiguous() * scale + st["table"].t()[:, which].transpose(0, 1)
     s = s.masked_fill(hide, float("-inf"))
     top = s.amax(-1, keepdim=True)
     p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
@@ -317,7 +316,7 @@ def _run_attn(st):
     krows = st["k"].shape[0]
     out["dq"] = _unpad(dq.transpose(1, 2), q_off, rows).to(dt)
     out["dk"], out["dv"] = (_unpad(gather(x), k_off, krows).to(dt) for x in (dk, dv))
-    out["dtable"] = _by_bucket(st, ds, shift).to(dt)
+    out["dtable"] = _by_bucket(st, ds, shift)
     return out
 
 
