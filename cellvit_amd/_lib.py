@@ -117,7 +117,7 @@ SYMBOLS.update({
 
 class cv_rel_attn(C.Structure):
     _fields_ = ([(n, C.c_int32) for n in ("dtype", "n_seq", "heads", "kv_heads", "head_dim", "max_q", "max_k", "causal", "num_buckets", "span")]
-                + [("scale", C.c_float), ("table_dtype", C.c_int32), ("zero_rest", C.c_int32), ("reserved", C.c_int32)]
+                + [("scale", C.c_float), ("table_dtype", C.c_int32), ("zero_rest", C.c_int32), ("lo_f32", C.c_int32)]
                 + [(n, C.c_int64) for n in ("rows_q", "rows_k", "q_seq", "q_row", "q_head", "k_seq", "k_row", "k_head", "v_seq", "v_row", "v_head",
                                             "o_seq", "o_row", "o_head", "do_seq", "do_row", "do_head")]
                 + [(n, C.c_void_p) for n in ("q", "k", "v", "q_off", "k_off", "table", "map", "out", "lse", "out_lo", "dout", "dq", "dk", "dv",

@@ -24,7 +24,7 @@ struct RelAttn {                                  // kernel argument
     int spread;                                   // sequences of unknown lengths: deal (sequence, key head) pairs to the XCDs in turn
     int win;                                      // offsets of one head's bias window in LDS
     float c;                                      // scale * log2 e
-    float* part_o; float* part_ml;                // partial results of the splits
+    float* part_o; float* part_rest; float* part_ml;       // partial results of the splits
     float* delta; float* amax; int n_amax;        // backward: (lse, +inf where a row saw no key; rowsum(dout * out)) of the rows, maxima of |dout|
     float* dpart; int units;                      // backward: partial table gradients
 };
@@ -245,14 +245,43 @@ int64_t rel_attention_bwd_tiles(const cv_rel_attn& a);
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
-// four or eight neighbouring results: rounded, and what the rounding took
-template <typename T, int N, typename V> __device__ __forceinline__ void store_rounded(T* dst, T* lo, const V& x) {
+// four or eight neighbouring results, rounded
+template <typename T, int N, typename V> __device__ __forceinline__ void store_rounded(T* dst, const V& x) {
     typedef T tn __attribute__((ext_vector_type(N)));
-    tn v, rest;
+    tn v;
 #pragma unroll
-    for (int j = 0; j < N; ++j) { v[j] = (T)x[j]; rest[j] = (T)(x[j] - (float)v[j]); }
+    for (int j = 0; j < N; ++j) v[j] = (T)x[j];
     *reinterpret_cast<tn*>(dst) = v;
-    if (lo) *reinterpret_cast<tn*>(lo) = rest;
+}
+// What rounding took from four neighbouring results that end up as x: their own last one, and `rest` that the rounding of P had taken before
+template <typename T, typename V> __device__ __forceinline__ void store_rest(const cv_rel_attn& a, long at, const V& x, const f32x4& rest) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    f32x4 lo;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lo[j] = (x[j] - (float)(T)x[j]) + rest[j];
+    if (a.lo_f32) { *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.out_lo) + at) = lo; return; }
+    t4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (T)lo[j];
+    *reinterpret_cast<t4*>(reinterpret_cast<T*>(a.out_lo) + at) = v;
+}
+// P for the product with V is rounded to T.  The backward's D = rowsum(dout out) goes into every dS of a row, so what that rounding takes from a row moves all of
+// them one way, and a bucket of the table's gradient collects it from its rows: 2e-4 (fp16) to 2e-3 (bf16) of a table's gradient at 1500 keys.  A forward
+// that is asked for `out_lo` (REST) sums what is left of P, too, in accumulators of its own, so that `out` keeps its bits: one more part of 11 bits in fp16, on
+// a scale of 2^12 (above the subnormals), two of 8 bits in bf16 (one would leave 1e-6 .. 6e-6).  Then the table's gradient is good to fp32.
+template <typename T> struct Rest;
+template <> struct Rest<half_t> { static constexpr int PARTS = 1; static constexpr float UP = 4096.f; };
+template <> struct Rest<bhalf_t> { static constexpr int PARTS = 2; static constexpr float UP = 1.f; };
+template <> struct Rest<float> { static constexpr int PARTS = 0; static constexpr float UP = 1.f; };
+// the next part of what is left of a block of P; `part`: the one taken last (UP is 1 where there is more than one)
+template <typename T> __device__ __forceinline__ v8<T> next_part(f32x4& a, f32x4& b, const v8<T>& part) {
+    v8<T> f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        a[j] -= (float)part[j]; b[j] -= (float)part[4 + j];
+        f[j] = (T)(a[j] * Rest<T>::UP); f[4 + j] = (T)(b[j] * Rest<T>::UP);
+    }
+    return f;
 }
 
 // The four lane groups (lanes 16 g4 .. 16 g4 + 15) hold parts of one column: their maximum / sum, in every lane.  The swaps exchange rows of 16, then

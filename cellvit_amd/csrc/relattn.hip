@@ -13,11 +13,13 @@ namespace {
 // two waves and all fragments ahead); wider ones have registers for two waves at most.
 // 8 x 16 heads x 4096 x 80 fp16: 880 us, 780 TFLOP/s; bound by issue: a 16 x 16 block takes a SIMD 235 cycles, 88 of products (heads padded to 96 in the
 // first) and about 130 of VALU, half of that the exponentials; the two waves of a SIMD overlap them little.
-template <typename T, int DT, int MQ, int BK>
-__global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const RelAttn k) {
+// REST (training): the sums of what rounding P left, too; a second set of accumulators leaves two waves a SIMD for heads up to 64 (the third would spill).
+template <typename T, int DT, int MQ, int BK, bool REST>
+__global__ __launch_bounds__(256, DT > 64 || REST ? 2 : 3) void rel_attn_kernel(const RelAttn k) {
     typedef Dims<DT> Dm;
     constexpr bool WIDE = DT > 64;
-    constexpr int NB = BK / 16, VA = WIDE ? NB / 2 : 1, PT = pitch_of<T>(Dm::W);
+    constexpr bool LEAN = REST && MQ * DT > 160;                            // two sets of accumulators: no registers for fragments read ahead
+    constexpr int NB = BK / 16, VA = LEAN ? 0 : WIDE ? NB / 2 : 1, PT = pitch_of<T>(Dm::W);
     extern __shared__ __attribute__((aligned(32))) char lds[];
     const cv_rel_attn& a = k.a;
     T* tiles = reinterpret_cast<T*>(lds);                                    // K, V; K, V
@@ -61,13 +63,16 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
     }
     if (D < Dm::W) zero_pad_columns<T, Dm::W>(tiles, 4 * BK, PT, D);
 
-    f32x4 o[MQ][Dm::ND];
+    f32x4 o[MQ][Dm::ND], rest[REST ? MQ : 1][Dm::ND];
     float mref[MQ], l[MQ];                                                   // reference exponent (base 2), lane's part of the sum
 #pragma unroll
     for (int m = 0; m < MQ; ++m) {
         mref[m] = NEG_INF; l[m] = 0.f;
 #pragma unroll
-        for (int d = 0; d < Dm::ND; ++d) o[m][d] = (f32x4)(0.f);
+        for (int d = 0; d < Dm::ND; ++d) {
+            o[m][d] = (f32x4)(0.f);
+            if constexpr (REST) rest[m][d] = (f32x4)(0.f);
+        }
     }
     const int krb = (int)a.k_row * (int)sizeof(T), vrb = (int)a.v_row * (int)sizeof(T);
     Stage<T, BK, Dm::W> sk, sv;
@@ -119,10 +124,14 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
             f32x4 sc[NB][MQ];
             float bc[MQ];                                                    // bias of a far tile: one exponent a row
             v8<T> kf[NB][Dm::KS];
+            const auto read_key = [&](int n, int ks) { return frag_row(kt + (n * 16 + li) * PT + ks * 32 + g4 * 8); };
+            const auto key = [&](int n, int ks) { return LEAN ? read_key(n, ks) : kf[n][ks]; };
+            if constexpr (!LEAN) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+                for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int ks = 0; ks < Dm::KS; ++ks) kf[n][ks] = frag_row(kt + (n * 16 + li) * PT + ks * 32 + g4 * 8);
+                    for (int ks = 0; ks < Dm::KS; ++ks) kf[n][ks] = read_key(n, ks);
+            }
             if (near(k0)) {
 #pragma unroll
                 for (int m = 0; m < MQ; ++m) {
@@ -134,15 +143,15 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
 #pragma unroll
                         for (int r = 0; r < 4; ++r) sc[n][m][r] = sp[n * 16 + r];
                 }
-                if constexpr (WIDE) ahead<T>();
+                if constexpr (WIDE && !LEAN) ahead<T>();
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int ks = 0; ks < Dm::KS; ++ks)
 #pragma unroll
-                        for (int m = 0; m < MQ; ++m) sc[n][m] = Seq<T>::mma(kf[n][ks], qf[m][ks], sc[n][m]);
+                        for (int m = 0; m < MQ; ++m) sc[n][m] = Seq<T>::mma(key(n, ks), qf[m][ks], sc[n][m]);
             } else {
-                if constexpr (WIDE) ahead<T>();
+                if constexpr (WIDE && !LEAN) ahead<T>();
 #pragma unroll
                 for (int m = 0; m < MQ; ++m) bc[m] = k0 >= phi ? far_hi[m] : far_lo[m];
 #pragma unroll
@@ -150,14 +159,14 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
 #pragma unroll
                     for (int ks = 0; ks < Dm::KS; ++ks)
 #pragma unroll
-                        for (int m = 0; m < MQ; ++m) sc[n][m] = Seq<T>::mma(kf[n][ks], qf[m][ks], ks ? sc[n][m] : (f32x4)(0.f));
+                        for (int m = 0; m < MQ; ++m) sc[n][m] = Seq<T>::mma(key(n, ks), qf[m][ks], ks ? sc[n][m] : (f32x4)(0.f));
             }
-            v8<T> vf[VA][Dm::ND];                                            // on their way behind the exponentials
+            v8<T> vf[VA ? VA : 1][Dm::ND];                                   // on their way behind the exponentials
 #pragma unroll
             for (int u = 0; u < VA; ++u)
 #pragma unroll
                 for (int d = 0; d < Dm::ND; ++d) vf[u][d] = frag_col(vt, PT, u * 32, d * 16, g4, li);
-            ahead<T>();
+            if constexpr (!LEAN) ahead<T>();
             if (k0 > whole) {
 #pragma unroll
                 for (int m = 0; m < MQ; ++m) {
@@ -185,7 +194,10 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
                     mref[m] = up;
                     l[m] *= f;
 #pragma unroll
-                    for (int d = 0; d < Dm::ND; ++d) o[m][d] *= f;
+                    for (int d = 0; d < Dm::ND; ++d) {
+                        o[m][d] *= f;
+                        if constexpr (REST) rest[m][d] *= f;
+                    }
                 }
                 const float sub = bc[m] - (mref[m] == NEG_INF ? 0.f : mref[m]);
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -201,14 +213,26 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
             }
 #pragma unroll
             for (int u = 0; u < NB / 2; ++u) {
-                v8<T> pf[MQ];
+                v8<T> pf[MQ], rf[REST ? Rest<T>::PARTS : 1][MQ];
 #pragma unroll
-                for (int m = 0; m < MQ; ++m) pf[m] = frag_acc<T>(sc[2 * u][m], sc[2 * u + 1][m]);  // p rounded to T once, for the product only
+                for (int m = 0; m < MQ; ++m) {
+                    pf[m] = frag_acc<T>(sc[2 * u][m], sc[2 * u + 1][m]);     // p rounded to T once, for the product only
+                    if constexpr (REST) {
+#pragma unroll
+                        for (int x = 0; x < Rest<T>::PARTS; ++x) rf[x][m] = next_part<T>(sc[2 * u][m], sc[2 * u + 1][m], x ? rf[x ? x - 1 : 0][m] : pf[m]);
+                    }
+                }
 #pragma unroll
                 for (int d = 0; d < Dm::ND; ++d) {
                     const v8<T> v = u < VA ? vf[u < VA ? u : 0][d] : frag_col(vt, PT, u * 32, d * 16, g4, li);
 #pragma unroll
                     for (int m = 0; m < MQ; ++m) o[m][d] = Seq<T>::mma(v, pf[m], o[m][d]);
+                    if constexpr (REST) {
+#pragma unroll
+                        for (int x = 0; x < Rest<T>::PARTS; ++x)
+#pragma unroll
+                            for (int m = 0; m < MQ; ++m) rest[m][d] = Seq<T>::mma(v, rf[x][m], rest[m][d]);
+                    }
                 }
             }
         }
@@ -231,17 +255,23 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
             if (g4 == 0) { k.part_ml[pr * 2] = mref[m]; k.part_ml[pr * 2 + 1] = sum; }
 #pragma unroll
             for (int d = 0; d < Dm::ND; ++d)
-                if (d * 16 + g4 * 4 < D) *reinterpret_cast<f32x4*>(k.part_o + pr * D + d * 16 + g4 * 4) = o[m][d];
+                if (d * 16 + g4 * 4 < D) {
+                    *reinterpret_cast<f32x4*>(k.part_o + pr * D + d * 16 + g4 * 4) = o[m][d];
+                    if constexpr (REST) *reinterpret_cast<f32x4*>(k.part_rest + pr * D + d * 16 + g4 * 4) = rest[m][d];
+                }
             continue;
         }
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;    // an empty row: zeros; NaN stays NaN
         if (a.lse && g4 == 0) a.lse[row] = sum > 0.f ? mref[m] + log2_hw(sum) : sum == 0.f ? NEG_INF : sum;
         T* ob = reinterpret_cast<T*>(a.out) + (a.q_off ? (qr.row0 + qi) * a.o_row : s * a.o_seq + qi * a.o_row) + h * a.o_head;
-        T* lo = a.out_lo ? reinterpret_cast<T*>(a.out_lo) + row * D : nullptr;
 #pragma unroll
         for (int d = 0; d < Dm::ND; ++d) {
             const int c = d * 16 + g4 * 4;
-            if (c < D) store_rounded<T, 4>(ob + c, lo ? lo + c : nullptr, o[m][d] * inv);
+            if (c >= D) continue;
+            f32x4 x = o[m][d] * inv;
+            settle(x);                                                       // one value for both: else the product is rounded to T at once in one of them
+            store_rounded<T, 4>(ob + c, x);
+            if (a.out_lo) store_rest<T>(a, row * D + c, x, REST ? rest[REST ? m : 0][d] * (inv / Rest<T>::UP) : (f32x4)(0.f));
         }
     }
 }
@@ -250,7 +280,7 @@ __global__ __launch_bounds__(256, DT > 64 ? 2 : 3) void rel_attn_kernel(const Re
 // waited for between waves until the end.  K goes from memory to registers as the product reads it, V through the wave's own piece of LDS (it is
 // read transposed); the loads of a wave's next run are issued as soon as the registers of this one are free.  Bound by HBM: K and V once
 // (16 ragged contexts to 32768, 4 key heads of 128, bf16: 116 us, 4.2 TB/s; 86 % of a copy's rate).
-template <typename T, int DT>
+template <typename T, int DT, bool REST>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DT > 96 ? 1 : 2) void rel_attn_few_kernel(const RelAttn k) {
     typedef Dims<DT> Dm;
     constexpr int KB = 32, PT = pitch_of<T>(Dm::W), E = 16 / sizeof(T), NV = KB * (Dm::W / E) / 64, HALVES = sizeof(T) / 2;
@@ -325,9 +355,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DT > 96 ? 1 : 2) void rel_at
     const int lim = a.causal && pos < kr.len - 1 ? pos : kr.len - 1;
     const int whole = a.causal && plo + 1 < kr.len ? plo + 1 - KB : kr.len - KB;
 
-    f32x4 o[Dm::ND];
+    f32x4 o[Dm::ND], rest[REST ? Dm::ND : 1];
 #pragma unroll
-    for (int d = 0; d < Dm::ND; ++d) o[d] = (f32x4)(0.f);
+    for (int d = 0; d < Dm::ND; ++d) {
+        o[d] = (f32x4)(0.f);
+        if constexpr (REST) rest[d] = (f32x4)(0.f);
+    }
     float mref = NEG_INF, l = 0.f;
 #pragma unroll
     for (int ks = 0; ks < Dm::KS; ++ks) settle(qf[ks]);
@@ -364,7 +397,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DT > 96 ? 1 : 2) void rel_at
             mref = up;
             l *= f;
 #pragma unroll
-            for (int d = 0; d < Dm::ND; ++d) o[d] *= f;
+            for (int d = 0; d < Dm::ND; ++d) {
+                o[d] *= f;
+                if constexpr (REST) rest[d] *= f;
+            }
         }
         const float sub = bc - (mref == NEG_INF ? 0.f : mref);
 #pragma unroll
@@ -377,18 +413,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DT > 96 ? 1 : 2) void rel_at
         if (next < kend) fetch_v(next);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
         const v8<T> pf = frag_acc<T>(sc[0], sc[1]);
+        v8<T> rf[REST ? Rest<T>::PARTS : 1];
+        if constexpr (REST) {
 #pragma unroll
-        for (int d = 0; d < Dm::ND; ++d) o[d] = Seq<T>::mma(frag_col(vt, PT, 0, d * 16, g4, li), pf, o[d]);
+            for (int x = 0; x < Rest<T>::PARTS; ++x) rf[x] = next_part<T>(sc[0], sc[1], x ? rf[x ? x - 1 : 0] : pf);
+        }
+#pragma unroll
+        for (int d = 0; d < Dm::ND; ++d) {
+            const v8<T> v = frag_col(vt, PT, 0, d * 16, g4, li);
+            o[d] = Seq<T>::mma(v, pf, o[d]);
+            if constexpr (REST) {
+#pragma unroll
+                for (int x = 0; x < Rest<T>::PARTS; ++x) rest[d] = Seq<T>::mma(v, rf[x], rest[d]);
+            }
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
     }
-    // join the waves: rows of D + 2 floats (sums, reference, weight) in the space of V
-    constexpr int RW = DT + 4;
+    // join the waves: rows of D + 2 floats (sums, reference, weight), and the sums of what is left of P, in the space of V
+    constexpr int RW = (REST ? 2 : 1) * DT + 4;
     float* join = reinterpret_cast<float*>(lds);
     const float sum = sum_over_groups(l);
     __syncthreads();
     float* mine = join + (wave * 16 + li) * RW;
 #pragma unroll
-    for (int d = 0; d < Dm::ND; ++d) *reinterpret_cast<f32x4*>(mine + d * 16 + g4 * 4) = o[d];
+    for (int d = 0; d < Dm::ND; ++d) {
+        *reinterpret_cast<f32x4*>(mine + d * 16 + g4 * 4) = o[d];
+        if constexpr (REST) *reinterpret_cast<f32x4*>(mine + DT + 4 + d * 16 + g4 * 4) = rest[d];
+    }
     if (g4 == 0) { mine[DT] = mref; mine[DT + 1] = sum; }
     __syncthreads();
     // 16 threads a row, 4 columns a thread a turn
@@ -407,16 +458,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DT > 96 ? 1 : 2) void rel_at
     }
     T* ob = reinterpret_cast<T*>(a.out) + (a.q_off ? (qr.row0 + qrow) * a.o_row : s * a.o_seq + qrow * a.o_row) + h * a.o_head;
     for (int c = (threadIdx.x & 15) * 4; c < D; c += 64) {
-        f32x4 v = (f32x4)(0.f);
+        f32x4 v = (f32x4)(0.f), left = (f32x4)(0.f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v += m[w] * *reinterpret_cast<const f32x4*>(join + (w * 16 + row) * RW + c);
-        if (k.nsplit > 1) { *reinterpret_cast<f32x4*>(k.part_o + pr * D + c) = v; continue; }
-        store_rounded<T, 4>(ob + c, a.out_lo ? reinterpret_cast<T*>(a.out_lo) + out_row * D + c : nullptr, v * inv);
+        for (int w = 0; w < 4; ++w) {
+            v += m[w] * *reinterpret_cast<const f32x4*>(join + (w * 16 + row) * RW + c);
+            if constexpr (REST) left += m[w] * *reinterpret_cast<const f32x4*>(join + (w * 16 + row) * RW + DT + 4 + c);
+        }
+        if (k.nsplit > 1) {
+            *reinterpret_cast<f32x4*>(k.part_o + pr * D + c) = v;
+            if constexpr (REST) *reinterpret_cast<f32x4*>(k.part_rest + pr * D + c) = left;
+            continue;
+        }
+        f32x4 x = v * inv;
+        settle(x);                                                           // one value for both, as for many rows
+        store_rounded<T, 4>(ob + c, x);
+        if (a.out_lo) store_rest<T>(a, out_row * D + c, x, left * (inv / Rest<T>::UP));
     }
 }
 
 // Joins the key splits of a row: a wave a row, 16 lanes x 8 columns, four lanes of splits, in a fixed order (16 sequences x 16 heads, 32 splits: 9 us).
-template <typename T>
+template <typename T, bool REST>
 __global__ __launch_bounds__(256) void rel_attn_join_kernel(const RelAttn k) {
     const cv_rel_attn& a = k.a;
     const int lane = threadIdx.x & 63, c = (lane & 15) * 8, D = a.head_dim;
@@ -433,30 +494,41 @@ __global__ __launch_bounds__(256) void rel_attn_join_kernel(const RelAttn k) {
 #pragma unroll
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == NEG_INF ? 0.f : top;
-    float l = 0.f, o[8];
+    float l = 0.f, o[8], left[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = 0.f;
+    for (int j = 0; j < 8; ++j) o[j] = left[j] = 0.f;
+    const auto add = [&](float w, const float* src, float (&to)[8]) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(src), y = *reinterpret_cast<const f32x4*>(src + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { to[j] = fmaf(w, x[j], to[j]); to[4 + j] = fmaf(w, y[j], to[4 + j]); }
+    };
 #pragma unroll 4
     for (int i = lane >> 4; i < k.nsplit; i += 4) {
         const float w = exp2_hw(ml[i * 2] - ref);
         l = fmaf(w, ml[i * 2 + 1], l);
         if (c < D) {
-            const float* src = k.part_o + (pr * k.nsplit + i) * D + c;
-            const f32x4 x = *reinterpret_cast<const f32x4*>(src), y = *reinterpret_cast<const f32x4*>(src + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { o[j] = fmaf(w, x[j], o[j]); o[4 + j] = fmaf(w, y[j], o[4 + j]); }
+            add(w, k.part_o + (pr * k.nsplit + i) * D + c, o);
+            if constexpr (REST) add(w, k.part_rest + (pr * k.nsplit + i) * D + c, left);
         }
     }
     l = sum_over_groups(l);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = sum_over_groups(o[j]);
+    for (int j = 0; j < 8; ++j) {
+        o[j] = sum_over_groups(o[j]);
+        if constexpr (REST) left[j] = sum_over_groups(left[j]);
+    }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     if (a.lse && lane == 0) a.lse[(qr.row0 + qi) * a.heads + h] = l > 0.f ? ref + log2_hw(l) : l == 0.f ? NEG_INF : l;
     if (lane >= 16 || c >= D) return;
     T* ob = reinterpret_cast<T*>(a.out) + (a.q_off ? (qr.row0 + qi) * a.o_row : s * a.o_seq + qi * a.o_row) + h * a.o_head + c;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] *= inv;
-    store_rounded<T, 8>(ob, a.out_lo ? reinterpret_cast<T*>(a.out_lo) + ((qr.row0 + qi) * a.heads + h) * D + c : nullptr, o);
+    for (int j = 0; j < 8; ++j) { o[j] *= inv; settle(o[j]); left[j] *= inv / Rest<T>::UP; }
+    store_rounded<T, 8>(ob, o);
+    if (a.out_lo) {
+        const long at = ((qr.row0 + qi) * a.heads + h) * D + c;
+        store_rest<T>(a, at, f32x4{o[0], o[1], o[2], o[3]}, f32x4{left[0], left[1], left[2], left[3]});
+        store_rest<T>(a, at + 4, f32x4{o[4], o[5], o[6], o[7]}, f32x4{left[4], left[5], left[6], left[7]});
+    }
 }
 
 // keys a step: 64 (8 x 16 heads x 4096 x 80 fp16: 880 us, 912 with 32), or 32 where two buffers of 64 would leave little room for a second workgroup on a
@@ -496,28 +568,33 @@ FwdPlan fwd_plan(const cv_rel_attn& a) {
     return p;
 }
 
-template <typename T, int DT>
+template <typename T, int DT, bool REST>
 int few_launch(RelAttn& k, hipStream_t st) {
-    const size_t v = 4 * 32 * pitch_of<T>(Dims<DT>::W) * sizeof(T) + (k.a.table ? (size_t)k.G * k.a.num_buckets * 4 : 0), join = 64 * (DT + 4) * 4;
+    const size_t v = 4 * 32 * pitch_of<T>(Dims<DT>::W) * sizeof(T) + (k.a.table ? (size_t)k.G * k.a.num_buckets * 4 : 0), join = 64 * ((REST ? 2 : 1) * DT + 4) * 4;
     const size_t bytes = v > join ? v : join;
-    if (const int rc = allow_lds(&rel_attn_few_kernel<T, DT>, bytes)) return rc;
-    hipLaunchKernelGGL((rel_attn_few_kernel<T, DT>), dim3(part_grid(k)), dim3(256), bytes, st, k);
+    if (const int rc = allow_lds(&rel_attn_few_kernel<T, DT, REST>, bytes)) return rc;
+    hipLaunchKernelGGL((rel_attn_few_kernel<T, DT, REST>), dim3(part_grid(k)), dim3(256), bytes, st, k);
     return (int)hipGetLastError();
 }
 
-template <typename T, int DT, int MQ>
+template <typename T, int DT, int MQ, bool REST>
 int fwd_launch(RelAttn& k, hipStream_t st) {
     constexpr int BK = fwd_keys(sizeof(T) == 4, DT);
     const int G = k.G;
     if (k.a.table) k.win = window_size(k.a, G, BK + 64 * MQ / G);
     const size_t bytes = 4 * BK * pitch_of<T>(Dims<DT>::W) * sizeof(T) + (k.a.table ? (size_t)G * (k.a.num_buckets + k.win) * 4 : 0);
-    if (const int rc = allow_lds(&rel_attn_kernel<T, DT, MQ, BK>, bytes)) return rc;
-    hipLaunchKernelGGL((rel_attn_kernel<T, DT, MQ, BK>), dim3(part_grid(k)), dim3(256), bytes, st, k);
+    if (const int rc = allow_lds(&rel_attn_kernel<T, DT, MQ, BK, REST>, bytes)) return rc;
+    hipLaunchKernelGGL((rel_attn_kernel<T, DT, MQ, BK, REST>), dim3(part_grid(k)), dim3(256), bytes, st, k);
     return (int)hipGetLastError();
 }
 template <typename T, int DT, int MQ> int fwd_pick(RelAttn& k, hipStream_t st) {
-    if constexpr (MQ == 0) return few_launch<T, DT>(k, st);
-    else return fwd_launch<T, DT, MQ>(k, st);
+    if constexpr (sizeof(T) == 2)
+        if (k.a.out_lo) {
+            if constexpr (MQ == 0) return few_launch<T, DT, true>(k, st);
+            else return fwd_launch<T, DT, MQ, true>(k, st);
+        }
+    if constexpr (MQ == 0) return few_launch<T, DT, false>(k, st);
+    else return fwd_launch<T, DT, MQ, false>(k, st);
 }
 template <typename T, int MQ>
 int fwd_dim(RelAttn& k, hipStream_t st) {
@@ -534,12 +611,19 @@ template <typename T> int fwd_t(RelAttn& k, int mq, hipStream_t st) {
     else if constexpr (sizeof(T) == 2) rc = mq == 2 ? fwd_dim<T, 2>(k, st) : fwd_dim<T, 1>(k, st);
     else rc = fwd_dim<T, 1>(k, st);
     if (rc || k.nsplit == 1) return rc;
-    const long rows = (long)k.a.n_seq * k.a.max_q * k.a.heads;
-    hipLaunchKernelGGL((rel_attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, k);
+    const dim3 grid((unsigned)(((long)k.a.n_seq * k.a.max_q * k.a.heads + 3) / 4));
+    bool rest = false;
+    if constexpr (sizeof(T) == 2) {
+        rest = k.a.out_lo != nullptr;
+        if (rest) hipLaunchKernelGGL((rel_attn_join_kernel<T, true>), grid, dim3(256), 0, st, k);
+    }
+    if (!rest) hipLaunchKernelGGL((rel_attn_join_kernel<T, false>), grid, dim3(256), 0, st, k);
     return (int)hipGetLastError();
 }
 
 }  // namespace
+
+static bool keeps_rest(const cv_rel_attn& a) { return a.out_lo && a.dtype != CV_DTYPE_F32; }
 
 int64_t rel_attention_tiles(const cv_rel_attn& a, bool grad) {
     if (grad) return rel_attention_bwd_tiles(a);
@@ -551,7 +635,7 @@ int64_t rel_attention_fwd_ws(const cv_rel_attn& a) {
     if (a.n_seq == 0 || a.max_q == 0) return 0;
     const FwdPlan p = fwd_plan(a);
     if (p.nsplit == 1) return 0;
-    return (int64_t)a.n_seq * a.max_q * a.heads * p.nsplit * (a.head_dim + 2) * 4;
+    return (int64_t)a.n_seq * a.max_q * a.heads * p.nsplit * ((keeps_rest(a) ? 2 : 1) * a.head_dim + 2) * 4;
 }
 
 int launch_rel_attention(const cv_rel_attn& a, hipStream_t st) {
@@ -562,7 +646,9 @@ int launch_rel_attention(const cv_rel_attn& a, hipStream_t st) {
     k.c = a.scale * LOG2E;
     if (!a.table) k.a.num_buckets = 0;
     k.part_o = reinterpret_cast<float*>(a.ws);
-    k.part_ml = k.part_o + (long)a.n_seq * a.max_q * a.heads * p.nsplit * a.head_dim;
+    const long rows = (long)a.n_seq * a.max_q * a.heads * p.nsplit;
+    k.part_rest = k.part_o + rows * a.head_dim;
+    k.part_ml = k.part_rest + (keeps_rest(a) ? rows * a.head_dim : 0);
     return a.dtype == CV_DTYPE_F16 ? fwd_t<half_t>(k, p.mq, st) : a.dtype == CV_DTYPE_BF16 ? fwd_t<bhalf_t>(k, p.mq, st) : fwd_t<float>(k, p.mq, st);
 }
 

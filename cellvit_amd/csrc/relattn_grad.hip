@@ -126,7 +126,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
     const bool row = on && q < qr.len;
     float lse = __builtin_inff(), dl = 0.f, far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f;
     const long at_row = (qr.row0 + q) * a.heads + kvh * k.G + h0 + head;
-    const T* rest = reinterpret_cast<const T*>(a.out_lo) + at_row * D;
     float dot = 0.f;
 #pragma unroll
     for (int ks = 0; ks < Dm::KS; ++ks) {
@@ -136,16 +135,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
 #pragma unroll
         for (int j = 0; j < 8; ++j) dot = fmaf((float)df[ks][j], (float)of[j], dot);
         if (a.out_lo) {
-            const v8<T> lo = frag_global(rest, ks * 32 + g4 * 8, D, row);
+            if (a.lo_f32) {
+                const v8<float> lo = frag_global(reinterpret_cast<const float*>(a.out_lo) + at_row * D, ks * 32 + g4 * 8, D, row);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dot = fmaf((float)df[ks][j], (float)lo[j], dot);
+                for (int j = 0; j < 8; ++j) dot = fmaf((float)df[ks][j], lo[j], dot);
+            } else {
+                const v8<T> lo = frag_global(reinterpret_cast<const T*>(a.out_lo) + at_row * D, ks * 32 + g4 * 8, D, row);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dot = fmaf((float)df[ks][j], (float)lo[j], dot);
+            }
         }
     }
     dot = sum_over_groups(dot);                                              // D of the row; kept for the other kernel with the exponent to take off
+    // A 16-bit product is rounded towards minus infinity more often than up (-2.7e-8 a step of 64 in fp16 beside a result of 8: measured).  In a sum over a
+    // bucket such errors add up where dS itself cancels (2e-6 of a gradient at 1500 keys), so every other block of 16 positions works on -dO and D, and its
+    // sums change their sign at the end.
+    const bool minus = sizeof(T) == 2 && ((q0 >> 4) + blk & 1) != 0;
+    if (minus) {
+#pragma unroll
+        for (int ks = 0; ks < Dm::KS; ++ks) df[ks] = -df[ks];
+    }
     if (row) {
         const float e = a.lse[at_row] == NEG_INF ? __builtin_inff() : a.lse[at_row];       // a row that saw no key: every p is 0
         if (g4 == 0) { k.delta[at_row * 2] = e; k.delta[at_row * 2 + 1] = dot; }
-        lse = e - (float)ex; dl = -dot;                                      // the factor 2^ex rides in the exponent
+        lse = e - (float)ex; dl = minus ? dot : -dot;                                      // the factor 2^ex rides in the exponent
     }
     if (k.dpart) {
         for (int i = lane; i < nb; i += 64) bacc[i] = 0.f;
@@ -346,7 +359,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
         }
         __syncthreads();
     }
-    const float back = pow2i(-ex);
+    const float back = minus ? -pow2i(-ex) : pow2i(-ex);
     if (k.dpart) {
         if (on && open) close_sums((kend + BK - 1) / BK * BK);
         if (zone)

@@ -263,7 +263,7 @@ def _attn_setup(q, k, v, table, buckets, scale, causal, q_offsets, k_offsets, ma
     step = 4 if code == _lib.DTYPE_F32 else 8
     (q, sq), (k, sk), (v, sv) = _rows(q, step), _rows(k, step), _rows(v, step)
     scale = dim ** -0.5 if scale is None else float(scale)
-    head = (code, n_seq, heads, kv_heads, dim, max_q, max_k, 1 if causal else 0, nb, span, scale, tcode, zero_rest, 0, qs[0], ks[0], *sq, *sk, *sv)
+    head = (code, n_seq, heads, kv_heads, dim, max_q, max_k, 1 if causal else 0, nb, span, scale, tcode, zero_rest, 1, qs[0], ks[0], *sq, *sk, *sv)
     tail = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_offsets), _ptr(k_offsets), _ptr(table), _ptr(buckets))
     return _Attn(device, q, k, v, table, buckets, q_offsets, k_offsets, scale, bool(causal), max_q, max_k, n_seq, head, tail)
 
@@ -285,7 +285,7 @@ def _attn_forward(c: _Attn, out, train):
         out = (torch.empty_like if c.n_seq and c.max_q else torch.zeros_like)(q, memory_format=torch.contiguous_format)
     so = _rows(out, 1)[1]
     lse = torch.empty(q.shape[:-1], dtype=_F32, device=q.device) if train else None
-    lo = torch.empty_like(q, memory_format=torch.contiguous_format) if train and q.dtype is not _F32 else None
+    lo = torch.empty(q.shape, dtype=_F32, device=q.device) if train and q.dtype is not _F32 else None
     _attn_call(c, 0, (*so, 0, 0, 0), (out.data_ptr(), _ptr(lse), _ptr(lo), 0, 0, 0, 0, 0))
     return out, lse, lo
 

@@ -242,17 +242,19 @@ int cv_op_rel_bias_grad(int dtype, int table_dtype, const void* dbias, const int
  *   there are rows_q / rows_k in all; max_q / max_k bound the lengths (longer sequences are cut there).  Rows outside every sequence are left as they were.
  * A row that sees no key (or only biases of -inf) gets zeros and lse -inf.  Finite table entries act as if clamped to +-1.6e7 / log2(e): in
  * fp32 a larger one would absorb every score.  out: strides o_*; lse (may be NULL; the backward reads it and out): fp32 [rows, heads], BASE-2
- * logarithm of sum_j 2^(s_ij log2 e).  out_lo: `dtype`, contiguous [rows, heads, head_dim], what rounding took from out; a backward that is given it takes
- * rowsum(dout * out) from both (without it the gradients of rows that see few keys lose up to 10 % more to rounding).  dq / dk / dv: `dtype`, contiguous [rows, heads | kv_heads, head_dim].  The products take P and dS rounded
- * to `dtype`, so with a 16-bit dtype gradients, a fp32 table's too, are good to that type's
- * precision.  table NULL: no bias.  Keys and values of a sequence must be finite where they are hidden, too (a hidden key has weight 0, and 0 * inf
+ * logarithm of sum_j 2^(s_ij log2 e).  out_lo (may be NULL): contiguous [rows, heads, head_dim], fp32 if lo_f32, else `dtype`: what rounding took from out,
+ * P's before the product with V and the result's own.  A forward that writes it works longer; a backward that is given it takes rowsum(dout * out) from
+ * both.  dq / dk / dv: `dtype`, contiguous [rows, heads | kv_heads, head_dim].  The other products take P and dS rounded to `dtype`, so dq, dk and dv are good
+ * to that type's precision; dtable is summed before any rounding: with a fp32 out_lo it is good to fp32, without to `dtype`.  table NULL: no bias.  Keys
+ * and values of a sequence must be finite where they are hidden, too (a hidden key has weight 0, and 0 * inf
  * is no number); rows outside every sequence may hold anything.  out, dq, dk and dv overlap no other tensor of the call.  Limits beside
  * those: row strides (of out: any) up to 16 MiB, the heads of a group up to 1 GiB apart, 2^24 workgroups a launch.                     */
 typedef struct cv_rel_attn {
     int32_t dtype, n_seq, heads, kv_heads, head_dim, max_q, max_k, causal, num_buckets, span;
     float scale;                               /* 1e-6 .. 1e6 */
     int32_t table_dtype;
-    int32_t zero_rest, reserved;               /* zero_rest != 0: rows outside every sequence get zeros (out; dq, dk, dv) instead of staying as they were */
+    int32_t zero_rest, lo_f32;                 /* zero_rest != 0: rows outside every sequence get zeros (out; dq, dk, dv) instead of staying as they were;
+                                                  lo_f32 != 0: out_lo is fp32 (0: `dtype`) */
     int64_t rows_q, rows_k;                    /* packed rows (ignored without offsets) */
     int64_t q_seq, q_row, q_head, k_seq, k_row, k_head, v_seq, v_row, v_head, o_seq, o_row, o_head, do_seq, do_row, do_head;
     const void *q, *k, *v;

@@ -1,0 +1,81 @@
+"""GPU: gradients of the sequence operators held to what their types allow, each entry's errors added as independent ones (the bounds of test_gpu_seqops.py
+add the worst of every pair)."""
+import math
+
+import pytest
+import torch
+
+import seq_ref as R
+from test_gpu_seqops import BF16, F16, _map, _ops, _pack
+
+pytestmark = pytest.mark.gpu
+HALVES = pytest.mark.parametrize("dtype", [F16, BF16])
+
+
+def _dtable(q, k, v, do, table, m, scale, causal):
+    """(dtable, sum of squared errors) of one sequence in 64 bits, [buckets, heads].  Everything behind the table's gradient is held in fp32: a score's argument of
+    the exponential is below 16 and rounded three times (2^-21 each), so each P is off by less than 2^-19, each on its own; sums of a hundred terms a lane, then
+    trees, add 2^-24 sqrt(100) of their size; D = dO . o is off by the same errors of P in the forward.  So an entry is off by 2^-19 times the root of
+    the sum over its pairs of (P A)^2, A = |dP| + |D|, and over its rows of (P of the row in the bucket)^2 sum (P dP)^2.  (P rounded to 16 bits in D would put
+    2^-9 / sqrt(3) or 2^-11 / sqrt(3) in the place of 2^-19 in the second.)"""
+    q, k, v, do, t = (x.cpu().double() for x in (q, k, v, do, table))
+    (lq, H, _), (lk, Hk, _) = q.shape, k.shape
+    nb = t.shape[0]
+    value, square = torch.zeros(nb, H, dtype=torch.float64), torch.zeros(nb, H, dtype=torch.float64)
+    if lq == 0 or lk == 0:
+        return value, square
+    plane = R.bucket_plane(m, lq, lk)
+    flat = plane.reshape(-1)
+    for h in range(H):
+        g = h // (H // Hk)
+        s = scale * q[:, h] @ k[:, g].T + t[:, h][plane]
+        if causal:
+            s = s.masked_fill(torch.arange(lk)[None] > torch.arange(lq)[:, None] + lk - lq, -math.inf)
+        lse = torch.logsumexp(s, 1, keepdim=True)
+        p = torch.where(lse == -math.inf, torch.zeros(()).double(), torch.exp(s - lse.clamp(min=-1e300)))
+        dp = do[:, h] @ v[:, g].T
+        d = (p * dp).sum(1, keepdim=True)
+        value[:, h].index_add_(0, flat, (p * (dp - d)).reshape(-1))
+        square[:, h].index_add_(0, flat, (p * (dp.abs() + d.abs())).square().reshape(-1))
+        mass = torch.zeros(lq, nb, dtype=torch.float64).scatter_add_(1, plane, p)
+        square[:, h] += (mass.square() * (p * dp).square().sum(1, keepdim=True)).sum(0)
+    return value, square
+
+
+@HALVES
+@pytest.mark.parametrize("lens,heads,kv,dim,causal,nb,span,packed", [
+    ([(257, 257)] * 2, 3, 3, 64, False, 32, 128, False),
+    ([(700, 700)], 2, 2, 64, False, 32, 128, False),
+    ([(300, 411)], 4, 2, 128, True, 64, 200, False),
+    ([(3, 700)], 4, 2, 80, True, 32, 64, False),                             # few rows: the keys are split and the parts joined
+    ([(5, 40)], 2, 1, 128, False, 16, 20, False),                            # few rows, one part
+    ([(20, 1500)], 1, 1, 32, False, 32, 128, False),                         # more rows, split keys
+    ([(130, 130), (0, 0), (7, 90), (1, 1), (200, 64)], 6, 6, 64, True, 32, 128, True),
+    ([(400, 400)] * 8, 16, 16, 32, False, 32, 128, False),                   # 32 rows a wave
+    ([(390, 390)] * 8, 16, 16, 128, True, 32, 300, False),
+    ([(260, 260)] * 3, 126, 42, 96, False, 16, 64, False),                   # 32 rows a wave, tiles of 126 rows
+])
+def test_a_float32_tables_gradient_is_good_to_float32(dtype, lens, heads, kv, dim, causal, nb, span, packed):
+    ops = _ops()
+    g = torch.Generator().manual_seed(31)
+    rows = lambda i, h: [torch.randn(n[i], h, dim, generator=g).to(dtype) for n in lens]  # noqa: E731
+    qs, ks, vs, dos = rows(0, heads), rows(1, kv), rows(1, kv), rows(0, heads)
+    table, m = torch.randn(nb, heads, generator=g), _map(nb, span, not causal)
+    kw = dict(causal=causal)
+    if packed:
+        (q, qo), (k, ko) = _pack(qs, 2), _pack(ks, 2)
+        v, do = _pack(vs, 2)[0], _pack(dos, 2)[0]
+        kw.update(q_offsets=qo, k_offsets=ko, max_q=max(a for a, _ in lens), max_k=max(b for _, b in lens))
+    else:
+        q, k, v, do = (torch.stack(x).cuda() for x in (qs, ks, vs, dos))
+    out, saved = ops.rel_attention_train(q, k, v, table.cuda(), m.cuda(), **kw)
+    with torch.no_grad():
+        assert torch.equal(out, ops.rel_attention(q, k, v, table.cuda(), m.cuda(), **kw))
+    got = ops.rel_attention_grad(saved, do)[3]
+    assert got.dtype == torch.float32
+    parts = [_dtable(a, b, c, d, table, m, dim ** -0.5, causal) for a, b, c, d in zip(qs, ks, vs, dos)]
+    want, bound = sum(p[0] for p in parts), 2.0 ** -19 * sum(p[1] for p in parts).sqrt()
+    off = (got.double().cpu() - want).abs()
+    # an entry's error is a sum of independent ones: four times its size is allowed, once for their norm
+    assert bool((off <= 4 * bound + 1e-30).all()), f"worst {float((off / bound.clamp(min=1e-30)).max()):.1f} x its size"
+    assert float(off.norm()) <= float(bound.norm())
