@@ -10,6 +10,7 @@ using namespace cva;
 namespace {
 
 constexpr int64_t LAUNCH_GROUPS = 1 << 24;       // workgroups of 256 threads
+constexpr int64_t MOST_ROWS = 0x7fffffff;        // offsets are int32
 
 bool dtype_ok(int d) { return d == CV_DTYPE_F16 || d == CV_DTYPE_BF16 || d == CV_DTYPE_F32; }
 int size_of(int d) { return d == CV_DTYPE_F32 ? 4 : 2; }
@@ -61,8 +62,8 @@ int check_plane(const char* fn, int dtype, int heads, int q_len, int k_len) {
     return CV_OK;
 }
 
-int check_attn(const cv_rel_attn* a, bool grad) {
-    const char* fn = grad ? "cv_op_rel_attention_grad" : "cv_op_rel_attention";
+// everything that the plans and the workspace sizes rely on
+int check_attn_shape(const char* fn, const cv_rel_attn* a, bool grad) {
     if (!a) REFUSE(CV_ERR_INVALID, "%s: null argument", fn);
     if (!dtype_ok(a->dtype)) REFUSE(CV_ERR_INVALID, "%s: dtype must be f16, bf16 or f32", fn);
     if (a->n_seq < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 65536)
@@ -71,13 +72,26 @@ int check_attn(const cv_rel_attn* a, bool grad) {
     if (G > 32) REFUSE(CV_ERR_UNSUPPORTED, "%s: at most 32 query heads share a key head (got %d)", fn, G);
     if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8) REFUSE(CV_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 up to 128 (got %d)", fn, a->head_dim);
     if (a->max_q < 0 || a->max_k < 0 || (int64_t)a->max_q * G > (1 << 28) || a->max_k > (1 << 28)) REFUSE(CV_ERR_INVALID, "%s: bad lengths (max_q %d, max_k %d)", fn, a->max_q, a->max_k);
+    if ((a->q_off && a->rows_q < 0) || (a->k_off && a->rows_k < 0)) REFUSE(CV_ERR_INVALID, "%s: negative number of rows", fn);
+    if ((a->q_off && a->rows_q > MOST_ROWS) || (a->k_off && a->rows_k > MOST_ROWS)) REFUSE(CV_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 packed rows", fn);
+    if ((a->table || a->dtable) && (a->num_buckets < 1 || a->num_buckets > 256)) REFUSE(CV_ERR_INVALID, "%s: num_buckets must be 1 .. 256 (got %d)", fn, a->num_buckets);
+    if ((a->table || a->dtable) && (a->span < 0 || a->span > 65536)) REFUSE(CV_ERR_INVALID, "%s: span must be 0 .. 65536 (got %d)", fn, a->span);
+    // a launch has less than 2^32 threads, 256 a workgroup
+    const int64_t pairs = (int64_t)a->kv_heads * a->n_seq;
+    if (pairs >= LAUNCH_GROUPS || (rel_attention_tiles(*a, grad) * ((pairs + 7) & ~7LL)) >= LAUNCH_GROUPS) REFUSE(CV_ERR_UNSUPPORTED, "%s: too many tiles for one launch", fn);
+    return CV_OK;
+}
+
+int check_attn(const cv_rel_attn* a, bool grad) {
+    const char* fn = grad ? "cv_op_rel_attention_grad" : "cv_op_rel_attention";
+    if (const int rc = check_attn_shape(fn, a, grad)) return rc;
+    const int G = a->heads / a->kv_heads;
     if (!(a->scale >= 1e-6f && a->scale <= 1e6f)) REFUSE(CV_ERR_INVALID, "%s: scale must lie in 1e-6 .. 1e6", fn);
     if (a->table) {
         const int rc = check_map(fn, a->dtype, a->table_dtype, a->map, a->num_buckets, a->span);
         if (rc) return rc;
     }
     if (a->dtable && !a->table) REFUSE(CV_ERR_INVALID, "%s: dtable without a table", fn);
-    if ((a->q_off && a->rows_q < 0) || (a->k_off && a->rows_k < 0)) REFUSE(CV_ERR_INVALID, "%s: negative number of rows", fn);
     const int64_t e = 16 / size_of(a->dtype);
     const int64_t strides[] = {a->q_seq, a->q_row, a->q_head, a->k_seq, a->k_row, a->k_head, a->v_seq, a->v_row, a->v_head, a->o_seq, a->o_row, a->o_head};
     for (int64_t s : strides)
@@ -104,9 +118,6 @@ int check_attn(const cv_rel_attn* a, bool grad) {
         for (const void* p : more)
             if (!aligned(p, 16)) REFUSE(CV_ERR_INVALID, "%s: pointers must be 16-byte aligned", fn);
     }
-    // a launch has less than 2^32 threads, 256 a workgroup
-    const int64_t pairs = (int64_t)a->kv_heads * a->n_seq;
-    if (pairs >= LAUNCH_GROUPS || (rel_attention_tiles(*a, grad) * ((pairs + 7) & ~7LL)) >= LAUNCH_GROUPS) REFUSE(CV_ERR_UNSUPPORTED, "%s: too many tiles for one launch", fn);
     return CV_OK;
 }
 
@@ -180,12 +191,8 @@ extern "C" int cv_op_rel_bias_grad(int dtype, int table_dtype, const void* dbias
 }
 
 extern "C" int64_t cv_op_rel_attention_ws(const cv_rel_attn* a, int grad) {
-    if (!a) { cva_set_error("cv_op_rel_attention_ws: null argument"); return -1; }
-    cv_rel_attn c = *a;
-    if (!grad) c.dtable = nullptr;
-    if (!dtype_ok(c.dtype) || c.heads < 1 || c.kv_heads < 1 || c.heads % c.kv_heads || c.max_q < 0 || c.max_k < 0 || c.n_seq < 0 || c.rows_q < 0 ||
-        c.head_dim < 8 || c.head_dim > 128) { cva_set_error("cv_op_rel_attention_ws: bad sizes"); return -1; }
-    return grad ? rel_attention_bwd_ws(c) : rel_attention_fwd_ws(c);
+    if (const int rc = check_attn_shape("cv_op_rel_attention_ws", a, grad != 0)) return -rc;
+    return grad ? rel_attention_bwd_ws(*a) : rel_attention_fwd_ws(*a);
 }
 extern "C" int cv_op_rel_attention(const cv_rel_attn* a, void* stream) {
     const int rc = check_attn(a, false);

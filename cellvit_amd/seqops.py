@@ -273,6 +273,8 @@ def _attn_call(c: _Attn, grad: int, strides: tuple, ptrs: tuple) -> None:
     lib = _lib.load()
     a = _ATTN.pack(*c.head, *strides, *c.tail, *ptrs, 0, 0)
     need = lib.cv_op_rel_attention_ws(a, grad)
+    if need < 0:
+        _lib.check(-need)
     if need > 0:
         ws = torch.empty(need, dtype=torch.uint8, device=c.q.device)
         a = _ATTN.pack(*c.head, *strides, *c.tail, *ptrs, ws.data_ptr(), need)

@@ -270,7 +270,7 @@ typedef struct cv_rel_attn {
     void* ws;
     int64_t ws_bytes;
 } cv_rel_attn;
-int64_t cv_op_rel_attention_ws(const cv_rel_attn* a, int grad);      /* bytes, or -1: refused (cv_last_error says why) */
+int64_t cv_op_rel_attention_ws(const cv_rel_attn* a, int grad);      /* bytes, or refused: minus the status (cv_last_error says why) */
 int cv_op_rel_attention(const cv_rel_attn* a, void* stream);
 int cv_op_rel_attention_grad(const cv_rel_attn* a, void* stream);
 
