@@ -9,25 +9,26 @@
 namespace cva {
 namespace {
 
-// fp16: the largest |dO| of every workgroup's rows.  Rows outside every sequence hold anything and are left out.  16 lanes a row.
+// fp16: the largest |dO| of every workgroup's rows: a sequence for `parts` of them.  Rows that no sequence owns, those it was cut by among them, hold anything
+// and are left out.  16 lanes a row.
 template <typename T>
-__global__ __launch_bounds__(256) void rel_amax_kernel(const RelAttn k, long total) {
+__global__ __launch_bounds__(256) void rel_amax_kernel(const RelAttn k, int parts) {
     __shared__ float red[4];
     const cv_rel_attn& a = k.a;
-    const int c = (threadIdx.x & 15) * 8, D = a.head_dim;
-    long lo = 0, hi = total;
-    if (a.q_off) {
-        const long b = a.q_off[0], e = a.q_off[a.n_seq];
-        lo = (b < 0 ? 0 : b) * a.heads; hi = (e > a.rows_q ? a.rows_q : e) * a.heads;
-    }
+    const int c = (threadIdx.x & 15) * 8, D = a.head_dim, part = (int)blockIdx.x % parts;
     float top = 0.f;
-    if (c < D)
-        for (long row = lo + (long)blockIdx.x * 16 + (threadIdx.x >> 4); row < hi; row += (long)gridDim.x * 16) {
-            const long tok = row / a.heads, s = a.q_off ? 0 : tok / a.max_q, i = tok - s * a.max_q;
-            const v8<T> d = *reinterpret_cast<const v8<T>*>(reinterpret_cast<const T*>(a.dout) + s * a.do_seq + i * a.do_row + (row - tok * a.heads) * a.do_head + c);
+    for (int s = (int)blockIdx.x / parts; s < a.n_seq; s += (int)gridDim.x / parts) {
+        const SeqRange qr = seq_range(a.q_off, s, a.max_q, a.rows_q);
+        const T* base = reinterpret_cast<const T*>(a.dout) + (a.q_off ? qr.row0 * a.do_row : s * a.do_seq);
+        const long rows = (long)qr.len * a.heads;
+        if (c < D)
+            for (long row = (long)part * 16 + (threadIdx.x >> 4); row < rows; row += (long)parts * 16) {
+                const long i = row / a.heads;
+                const v8<T> d = *reinterpret_cast<const v8<T>*>(base + i * a.do_row + (row - i * a.heads) * a.do_head + c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)d[j]));
-        }
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)d[j]));
+            }
+    }
 #pragma unroll
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
@@ -757,7 +758,7 @@ __global__ __launch_bounds__(1024) void rel_dtable_kernel(const RelAttn k, int w
 // training step, 24 x 12 heads of 64: 660 us with two blocks, 612 with one; causal, heads of 128: 1305, with spills, and 1079).
 constexpr int BK_DQ = 32, BQ_DKV = 32;
 
-struct BwdPlan { int keys, ht, q_rt, q_tiles, k_tiles, n_amax; long rows, units; int64_t stat, amax, part; };
+struct BwdPlan { int keys, ht, q_rt, q_tiles, k_tiles, n_amax, amax_parts; long rows, units; int64_t stat, amax, part; };
 BwdPlan bwd_plan(const cv_rel_attn& a) {
     BwdPlan p;
     const int G = a.heads / a.kv_heads;
@@ -768,8 +769,9 @@ BwdPlan bwd_plan(const cv_rel_attn& a) {
     p.q_tiles = q_parts * ((G + p.ht - 1) / p.ht);
     p.k_tiles = (a.max_k + p.keys - 1) / p.keys;
     p.rows = a.q_off ? a.rows_q : (long)a.n_seq * a.max_q;
-    const long blocks = (p.rows * a.heads + 15) / 16;
-    p.n_amax = (int)(blocks < 1024 ? (blocks < 1 ? 1 : blocks) : 1024);
+    const long blocks = ((long)a.max_q * a.heads + 15) / 16, share = a.n_seq > 0 && a.n_seq < 1024 ? 1024 / a.n_seq : 1;        // of a sequence
+    p.amax_parts = (int)(blocks < share ? (blocks < 1 ? 1 : blocks) : share);
+    p.n_amax = (a.n_seq < 1 ? 1 : a.n_seq < 1024 ? a.n_seq : 1024) * p.amax_parts;
     p.units = (long)a.n_seq * q_parts * (p.q_rt / 16);
     const auto round = [](int64_t n) { return (n + 15) / 16 * 16; };
     p.stat = round(p.rows * a.heads * 8);
@@ -786,7 +788,7 @@ int bwd_launch(RelAttn& k, const BwdPlan& p, hipStream_t st) {
     const int G = k.G;
     int rc = 0;
     if constexpr (__is_same(T, half_t)) {
-        hipLaunchKernelGGL((rel_amax_kernel<T>), dim3(p.n_amax), dim3(256), 0, st, k, p.rows * a.heads);
+        hipLaunchKernelGGL((rel_amax_kernel<T>), dim3(p.n_amax), dim3(256), 0, st, k, p.amax_parts);
         if ((rc = (int)hipGetLastError())) return rc;
     }
     const size_t tabs = a.table ? (size_t)G * a.num_buckets : 0;

@@ -79,3 +79,29 @@ def test_a_float32_tables_gradient_is_good_to_float32(dtype, lens, heads, kv, di
     # an entry's error is a sum of independent ones: four times its size is allowed, once for their norm
     assert bool((off <= 4 * bound + 1e-30).all()), f"worst {float((off / bound.clamp(min=1e-30)).max()):.1f} x its size"
     assert float(off.norm()) <= float(bound.norm())
+
+
+@HALVES
+@pytest.mark.parametrize("junk", [math.nan, math.inf, 65504.0, -1e4])
+def test_what_cut_and_unowned_rows_hold_changes_no_gradient(dtype, junk):
+    """Sequences longer than max_q / max_k are cut there: the rest belongs to no sequence, nor do the rows before the first and behind the last."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(32)
+    mk = lambda n: torch.randn(n, 2, 64, generator=g).to(dtype)  # noqa: E731
+    q, k, v, do = mk(230), mk(260), mk(260), mk(230)
+    qo, ko = torch.tensor([5, 105, 105, 225], dtype=torch.int32), torch.tensor([3, 123, 133, 255], dtype=torch.int32)
+    table, m = torch.randn(16, 2, generator=g).cuda(), _map(16, 20, True).cuda()
+    lost_q, lost_k = torch.ones(230, dtype=torch.bool), torch.ones(260, dtype=torch.bool)
+    for a, b in zip(qo[:-1].tolist(), qo[1:].tolist()):
+        lost_q[a:min(b, a + 70)] = False
+    for a, b in zip(ko[:-1].tolist(), ko[1:].tolist()):
+        lost_k[a:min(b, a + 90)] = False
+    res = []
+    for fill in (0.0, junk):
+        a, b, c, d = (t.clone() for t in (q, k, v, do))
+        for t, lost in ((a, lost_q), (b, lost_k), (c, lost_k), (d, lost_q)):
+            t[lost] = fill
+        out, saved = ops.rel_attention_train(a.cuda(), b.cuda(), c.cuda(), table, m, q_offsets=qo.cuda(), k_offsets=ko.cuda(), max_q=70, max_k=90)
+        res.append([out, *ops.rel_attention_grad(saved, d.cuda())])
+    for x, y in zip(*res):
+        assert bool(torch.isfinite(y).all()) and torch.equal(x, y)
