@@ -25,7 +25,7 @@ struct RelAttn {                                  // kernel argument
     int win;                                      // offsets of one head's bias window in LDS
     float c;                                      // scale * log2 e
     float* part_o; float* part_rest; float* part_ml;       // partial results of the splits
-    float* delta; float* amax; int n_amax;        // backward: (lse, +inf where a row saw no key; rowsum(dout * out)) of the rows, maxima of |dout|
+    float* delta; float* amax; int n_amax;        // backward: (lse, +inf where a row saw no key; rowsum(dout * out)) of the rows, maxima of |dout| and |v|
     float* dpart; int units;                      // backward: partial table gradients
 };
 

@@ -2,53 +2,71 @@
 //   P = 2^(s - lse),  dV = P^T dO,  dP = dO V^T,  dS = P (dP - D),  D_i = dO_i . o_i,  dQ = scale dS K,  dK = scale dS^T Q,  dt[c] = sum dS over bucket c
 // Two kernels that each own what they write (dQ and the table's gradient by rows, dK and dV by keys), so no sum depends on scheduling; the price is
 // seven products where five would do.
-// fp16: dS is scaled by a power of two that brings max |dO| to 1/4 .. 1/2 (exact, taken out of the results), so that small gradients stay above
-// fp16's subnormals; |dS| <= max |dP| / 2 <= D max |V| / 4 then, so that values of up to 2000 are far from its end.
+// fp16: dS is scaled by a power of two from max |dO| and max |V| (exact, taken out of the results): ds_exponent.
 #include "relattn.h"
 
 namespace cva {
 namespace {
 
-// fp16: the largest |dO| of every workgroup's rows: a sequence for `parts` of them.  Rows that no sequence owns, those it was cut by among them, hold anything
-// and are left out.  16 lanes a row.
+// fp16: the largest |dO| and |V| of every workgroup's rows: a sequence for `parts` of them.  Rows that no sequence owns, those it was cut by among them, hold
+// anything and are left out.  16 lanes a row.
 template <typename T>
 __global__ __launch_bounds__(256) void rel_amax_kernel(const RelAttn k, int parts) {
-    __shared__ float red[4];
+    __shared__ float red[4][2];
     const cv_rel_attn& a = k.a;
     const int c = (threadIdx.x & 15) * 8, D = a.head_dim, part = (int)blockIdx.x % parts;
-    float top = 0.f;
-    for (int s = (int)blockIdx.x / parts; s < a.n_seq; s += (int)gridDim.x / parts) {
-        const SeqRange qr = seq_range(a.q_off, s, a.max_q, a.rows_q);
-        const T* base = reinterpret_cast<const T*>(a.dout) + (a.q_off ? qr.row0 * a.do_row : s * a.do_seq);
-        const long rows = (long)qr.len * a.heads;
+    const auto scan = [&](const T* base, int len, int heads, long step, long head, float top) {
+        const long rows = (long)len * heads;
         if (c < D)
             for (long row = (long)part * 16 + (threadIdx.x >> 4); row < rows; row += (long)parts * 16) {
-                const long i = row / a.heads;
-                const v8<T> d = *reinterpret_cast<const v8<T>*>(base + i * a.do_row + (row - i * a.heads) * a.do_head + c);
+                const long i = row / heads;
+                const v8<T> d = *reinterpret_cast<const v8<T>*>(base + i * step + (row - i * heads) * head + c);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)d[j]));
             }
+        return top;
+    };
+    float top[2] = {0.f, 0.f};
+    for (int s = (int)blockIdx.x / parts; s < a.n_seq; s += (int)gridDim.x / parts) {
+        const SeqRange qr = seq_range(a.q_off, s, a.max_q, a.rows_q), kr = seq_range(a.k_off, s, a.max_k, a.rows_k);
+        top[0] = scan(reinterpret_cast<const T*>(a.dout) + (a.q_off ? qr.row0 * a.do_row : s * a.do_seq), qr.len, a.heads, a.do_row, a.do_head, top[0]);
+        top[1] = scan(reinterpret_cast<const T*>(a.v) + (a.k_off ? kr.row0 * a.v_row : s * a.v_seq), kr.len, a.kv_heads, a.v_row, a.v_head, top[1]);
     }
 #pragma unroll
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int x = 32; x; x >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], x));
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][i] = top[i];
+    }
     __syncthreads();
-    if (threadIdx.x == 0) k.amax[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (threadIdx.x < 2) {
+        const int i = threadIdx.x;
+        k.amax[blockIdx.x * 2 + i] = fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i]));
+    }
 }
 
-// exponent e of the factor 2^e on dS (0 unless T is fp16); every thread of the workgroup must call it
+// exponent e of the factor 2^e on dS (0 unless T is fp16); every thread of the workgroup must call it.  |dP| <= D max |dO| max |V| =: B, so |dS| = P |dP - D| <= B / 2
+// (P (1 - P) <= 1/4, |dP - mean| of the others <= 2 B); B 2^e lies in 2^14 .. 2^15: nothing that fits fp16 overflows, and 2^28 lie between the largest dS and
+// the subnormals.
 template <typename T> __device__ __forceinline__ int ds_exponent(const RelAttn& k) {
     if constexpr (__is_same(T, half_t)) {
-        __shared__ float red[4];
-        float top = 0.f;
-        for (int i = threadIdx.x; i < k.n_amax; i += blockDim.x) top = fmaxf(top, k.amax[i]);
+        __shared__ float red[4][2];
+        float top[2] = {0.f, 0.f};
+        for (int i = threadIdx.x; i < k.n_amax; i += blockDim.x)
 #pragma unroll
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        if ((threadIdx.x & 63) == 0 && threadIdx.x < 256) red[threadIdx.x >> 6] = top;
+            for (int x = 0; x < 2; ++x) top[x] = fmaxf(top[x], k.amax[i * 2 + x]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int x = 32; x; x >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], x));
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][i] = top[i];
+        }
         __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        if (!(top > 0.f) || top > 65504.f) return 0;
-        return 125 - (int)((__float_as_uint(top) >> 23) & 0xff);             // top in [2^x, 2^(x+1)) -> [1/4, 1/2)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) top[i] = fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i]));
+        const float b = (float)k.a.head_dim * top[0] * top[1];
+        if (!(b > 0.f) || b > 3e38f) return 0;
+        return 141 - (int)((__float_as_uint(b) >> 23) & 0xff);               // b in [2^x, 2^(x+1)) -> [2^14, 2^15)
     }
     return 0;
 }
@@ -769,13 +787,14 @@ BwdPlan bwd_plan(const cv_rel_attn& a) {
     p.q_tiles = q_parts * ((G + p.ht - 1) / p.ht);
     p.k_tiles = (a.max_k + p.keys - 1) / p.keys;
     p.rows = a.q_off ? a.rows_q : (long)a.n_seq * a.max_q;
-    const long blocks = ((long)a.max_q * a.heads + 15) / 16, share = a.n_seq > 0 && a.n_seq < 1024 ? 1024 / a.n_seq : 1;        // of a sequence
+    const long most_q = (long)a.max_q * a.heads, most_k = (long)a.max_k * a.kv_heads;
+    const long blocks = ((most_q > most_k ? most_q : most_k) + 15) / 16, share = a.n_seq > 0 && a.n_seq < 1024 ? 1024 / a.n_seq : 1;        // of a sequence
     p.amax_parts = (int)(blocks < share ? (blocks < 1 ? 1 : blocks) : share);
     p.n_amax = (a.n_seq < 1 ? 1 : a.n_seq < 1024 ? a.n_seq : 1024) * p.amax_parts;
     p.units = (long)a.n_seq * q_parts * (p.q_rt / 16);
     const auto round = [](int64_t n) { return (n + 15) / 16 * 16; };
     p.stat = round(p.rows * a.heads * 8);
-    p.amax = round((int64_t)p.n_amax * 4);
+    p.amax = round((int64_t)p.n_amax * 8);
     p.part = a.dtable ? round(p.units * a.heads * (int64_t)a.num_buckets * 4) : 0;
     return p;
 }

@@ -105,3 +105,25 @@ def test_what_cut_and_unowned_rows_hold_changes_no_gradient(dtype, junk):
         res.append([out, *ops.rel_attention_grad(saved, d.cuda())])
     for x, y in zip(*res):
         assert bool(torch.isfinite(y).all()) and torch.equal(x, y)
+
+
+@HALVES
+@pytest.mark.parametrize("dscale,vscale,dim", [(0.01, 8000.0, 128), (0.02, 60000.0, 64), (100.0, 2.0, 64), (3e-5, 1.0, 64), (1.0, 1e-3, 32)])
+def test_gradients_that_fit_their_type_survive_large_and_small_values(dtype, dscale, vscale, dim):
+    """dout and v of one sign pattern, two keys: |dP| is dim dscale vscale, the largest there can be for these sizes, and |dS| up to half of it."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(33)
+    lq, lk = 6, 2
+    pattern = torch.randn(dim, generator=g).sign()
+    side = torch.tensor([1.0, -1.0]).view(lk, 1, 1)
+    q, k = (torch.randn(1, n, 1, dim, generator=g).to(dtype) for n in (lq, lk))
+    k = (k.float() * 0.1).to(dtype)
+    v = (pattern * side * vscale).to(dtype)[None]
+    do = (pattern.expand(1, lq, 1, dim) * dscale).to(dtype)
+    ref = R.attention(q[0], k[0], v[0], None, None, dim ** -0.5, False, do[0])
+    saved = ops.rel_attention_train(q.cuda(), k.cuda(), v.cuda())[1]
+    got = ops.rel_attention_grad(saved, do.cuda())
+    for name, x in zip(("dq", "dk", "dv"), got):
+        want, bound = ref[name]
+        assert bool(torch.isfinite(want.to(dtype)).all()) and bool(torch.isfinite(x).all()), name
+        assert bool(((x[0].double().cpu() - want).abs() <= bound).all()), name
