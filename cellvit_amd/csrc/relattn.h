@@ -25,7 +25,8 @@ struct RelAttn {                                  // kernel argument
     int win;                                      // offsets of one head's bias window in LDS
     float c;                                      // scale * log2 e
     float* part_o; float* part_rest; float* part_ml;       // partial results of the splits
-    float* delta; float* amax; int n_amax;        // backward: (lse, +inf where a row saw no key; rowsum(dout * out)) of the rows, maxima of |dout| and |v|
+    float* delta;                                 // backward: (lse, +inf where a row saw no key; rowsum(dout * out)) of the rows
+    int* row_exp; float* amax; int n_amax;        // fp16's backward: exponents of the rows' dS; max |v_j|^2 of a (sequence, key head) pair in n_amax parts
     float* dpart; int units;                      // backward: partial table gradients
 };
 

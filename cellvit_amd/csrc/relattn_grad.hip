@@ -2,79 +2,59 @@
 //   P = 2^(s - lse),  dV = P^T dO,  dP = dO V^T,  dS = P (dP - D),  D_i = dO_i . o_i,  dQ = scale dS K,  dK = scale dS^T Q,  dt[c] = sum dS over bucket c
 // Two kernels that each own what they write (dQ and the table's gradient by rows, dK and dV by keys), so no sum depends on scheduling; the price is
 // seven products where five would do.
-// fp16: dS is scaled by a power of two from max |dO| and max |V| (exact, taken out of the results): ds_exponent.
+// fp16: a row's dS is scaled by a power of two from |dO_i| and max |V_j| for the products (exact, taken out of the results): ds_exponent.
 #include "relattn.h"
 
 namespace cva {
 namespace {
 
-// fp16: the largest |dO| and |V| of every workgroup's rows: a sequence for `parts` of them.  Rows that no sequence owns, those it was cut by among them, hold
-// anything and are left out.  16 lanes a row.
+// fp16: the largest |V_j|^2 of a (sequence, key head) pair, in n_amax parts.  Rows that no sequence owns, those it was cut by among them, hold anything and are
+// left out.  16 lanes a row.
 template <typename T>
-__global__ __launch_bounds__(256) void rel_amax_kernel(const RelAttn k, int parts) {
-    __shared__ float red[4][2];
+__global__ __launch_bounds__(256) void rel_vnorm_kernel(const RelAttn k) {
+    __shared__ float red[4];
     const cv_rel_attn& a = k.a;
-    const int c = (threadIdx.x & 15) * 8, D = a.head_dim, part = (int)blockIdx.x % parts;
-    const auto scan = [&](const T* base, int len, int heads, long step, long head, float top) {
-        const long rows = (long)len * heads;
-        if (c < D)
-            for (long row = (long)part * 16 + (threadIdx.x >> 4); row < rows; row += (long)parts * 16) {
-                const long i = row / heads;
-                const v8<T> d = *reinterpret_cast<const v8<T>*>(base + i * step + (row - i * heads) * head + c);
+    const int c = (threadIdx.x & 15) * 8, D = a.head_dim, pair = (int)blockIdx.x / k.n_amax, part = (int)blockIdx.x - pair * k.n_amax;
+    const int s = pair / a.kv_heads, kvh = pair - s * a.kv_heads;
+    const SeqRange kr = seq_range(a.k_off, s, a.max_k, a.rows_k);
+    const T* vb = reinterpret_cast<const T*>(a.v) + (a.k_off ? kr.row0 * a.v_row : s * a.v_seq) + (long)kvh * a.v_head;
+    float top = 0.f;
+    for (int r0 = part * 16; r0 < kr.len; r0 += k.n_amax * 16) {
+        const int r = r0 + ((int)threadIdx.x >> 4);
+        const v8<T> d = frag_global(vb + (long)r * a.v_row, c, D, r < kr.len);
+        float n = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)d[j]));
-            }
-        return top;
-    };
-    float top[2] = {0.f, 0.f};
-    for (int s = (int)blockIdx.x / parts; s < a.n_seq; s += (int)gridDim.x / parts) {
-        const SeqRange qr = seq_range(a.q_off, s, a.max_q, a.rows_q), kr = seq_range(a.k_off, s, a.max_k, a.rows_k);
-        top[0] = scan(reinterpret_cast<const T*>(a.dout) + (a.q_off ? qr.row0 * a.do_row : s * a.do_seq), qr.len, a.heads, a.do_row, a.do_head, top[0]);
-        top[1] = scan(reinterpret_cast<const T*>(a.v) + (a.k_off ? kr.row0 * a.v_row : s * a.v_seq), kr.len, a.kv_heads, a.v_row, a.v_head, top[1]);
+        for (int j = 0; j < 8; ++j) n = fmaf((float)d[j], (float)d[j], n);
+#pragma unroll
+        for (int x = 8; x; x >>= 1) n += __shfl_xor(n, x);
+        top = fmaxf(top, n);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int x = 32; x; x >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], x));
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][i] = top[i];
-    }
+    for (int x = 32; x >= 16; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x < 2) {
-        const int i = threadIdx.x;
-        k.amax[blockIdx.x * 2 + i] = fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i]));
-    }
+    if (threadIdx.x == 0) k.amax[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// exponent e of the factor 2^e on dS (0 unless T is fp16); every thread of the workgroup must call it.  |dP| <= D max |dO| max |V| =: B, so |dS| = P |dP - D| <= B / 2
-// (P (1 - P) <= 1/4, |dP - mean| of the others <= 2 B); B 2^e lies in 2^14 .. 2^15: nothing that fits fp16 overflows, and 2^28 lie between the largest dS and
-// the subnormals.
-template <typename T> __device__ __forceinline__ int ds_exponent(const RelAttn& k) {
-    if constexpr (__is_same(T, half_t)) {
-        __shared__ float red[4][2];
-        float top[2] = {0.f, 0.f};
-        for (int i = threadIdx.x; i < k.n_amax; i += blockDim.x)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) top[x] = fmaxf(top[x], k.amax[i * 2 + x]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int x = 32; x; x >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], x));
-            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][i] = top[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) top[i] = fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i]));
-        const float b = (float)k.a.head_dim * top[0] * top[1];
-        if (!(b > 0.f) || b > 3e38f) return 0;
-        return 141 - (int)((__float_as_uint(b) >> 23) & 0xff);               // b in [2^x, 2^(x+1)) -> [2^14, 2^15)
-    }
-    return 0;
+// Exponent e of the factor 2^e on the dS of a row, b2 = |dO_i|^2 max |V_j|^2: |dP| <= B = sqrt(b2), so |dS| = P |dP - D| <= B / 2 (the other pairs' mean is at most
+// 2 B away and P (1 - P) <= 1/4); B 2^e lies in 2^14 .. 2^15, so nothing that fits fp16 overflows, and 2^28 lie between the largest dS and the
+// subnormals.  Each row of dQ has its own; dK takes the smallest of the rows its keys meet, tile by tile.
+constexpr int DS_FREE = 64;                                                  // a row of dS = 0
+__device__ __forceinline__ int ds_exponent(float b2) {
+    if (!(b2 > 0.f)) return DS_FREE;
+    return 14 - (((int)(__float_as_uint(b2) >> 23) - 127) >> 1);             // -50 for infinities
 }
+template <typename T> constexpr bool SCALED = __is_same(T, half_t);
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
 
 // waves a SIMD to leave registers for: fp32 fragments of wide heads need more than half of them
 template <typename T> constexpr int grad_waves(int DT) { return sizeof(T) == 4 && DT > 80 ? 1 : 2; }
 
+// the smaller of v and, where the row mask takes part, what CTRL brings from another lane
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_min(int v) {
+    const int w = __builtin_amdgcn_update_dpp(v, v, CTRL, ROWS, 0xf, false);
+    return w < v ? w : v;
+}
 template <int CTRL> __device__ __forceinline__ float dpp_shift(float v) {
     return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
@@ -139,7 +119,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
     int kend = kr.len;
     if (a.causal && phi + 1 < kend) kend = phi + 1 < 0 ? 0 : phi + 1;
 
-    const int ex = ds_exponent<T>(k);
+    float vmax = 0.f, own = 0.f;                                             // fp16: max |V_j|^2, |dO_i|^2
+    if constexpr (SCALED<T>) {
+        for (int i = lane; i < k.n_amax; i += 64) vmax = fmaxf(vmax, k.amax[(long)(s * a.kv_heads + kvh) * k.n_amax + i]);
+#pragma unroll
+        for (int x = 32; x; x >>= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, x));
+    }
     v8<T> qf[Dm::KS], df[Dm::KS];
     const int q = q0 + blk * 16 + li, pos = q + shift;
     const bool row = on && q < qr.len;
@@ -152,7 +137,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
         df[ks] = frag_global(db + q * a.do_row + head * a.do_head, ks * 32 + g4 * 8, D, row);
         const v8<T> of = frag_global(ob + q * a.o_row + head * a.o_head, ks * 32 + g4 * 8, D, row);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dot = fmaf((float)df[ks][j], (float)of[j], dot);
+        for (int j = 0; j < 8; ++j) {
+            dot = fmaf((float)df[ks][j], (float)of[j], dot);
+            if constexpr (SCALED<T>) own = fmaf((float)df[ks][j], (float)df[ks][j], own);
+        }
         if (a.out_lo) {
             if (a.lo_f32) {
                 const v8<float> lo = frag_global(reinterpret_cast<const float*>(a.out_lo) + at_row * D, ks * 32 + g4 * 8, D, row);
@@ -166,6 +154,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
         }
     }
     dot = sum_over_groups(dot);                                              // D of the row; kept for the other kernel with the exponent to take off
+    float up = 1.f, down = 1.f;                                              // factor on the row's dS for the product
+    if constexpr (SCALED<T>) {
+        const int ex = ds_exponent(sum_over_groups(own) * vmax);
+        if (row && g4 == 0) k.row_exp[at_row] = ex;
+        up = pow2i(ex); down = pow2i(-ex);
+    }
     // A 16-bit product is rounded towards minus infinity more often than up (-2.7e-8 a step of 64 in fp16 beside a result of 8: measured).  In a sum over a
     // bucket such errors add up where dS itself cancels (2e-6 of a gradient at 1500 keys), so every other block of 16 positions works on -dO and D, and its
     // sums change their sign at the end.
@@ -177,7 +171,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
     if (row) {
         const float e = a.lse[at_row] == NEG_INF ? __builtin_inff() : a.lse[at_row];       // a row that saw no key: every p is 0
         if (g4 == 0) { k.delta[at_row * 2] = e; k.delta[at_row * 2 + 1] = dot; }
-        lse = e - (float)ex; dl = minus ? dot : -dot;                                      // the factor 2^ex rides in the exponent
+        lse = e; dl = minus ? dot : -dot;
     }
     if (k.dpart) {
         for (int i = lane; i < nb; i += 64) bacc[i] = 0.f;
@@ -366,6 +360,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
             }
 #pragma unroll
             for (int u = 0; u < NB / 2; ++u) {
+                if constexpr (SCALED<T>) { sc[2 * u] *= up; sc[2 * u + 1] *= up; }
                 const v8<T> pf = frag_acc<T>(sc[2 * u], sc[2 * u + 1]);      // dS rounded to T once, for the product only
 #pragma unroll
                 for (int d = 0; d < Dm::ND; ++d) o[d] = Seq<T>::mma(kc[u][d], pf, o[d]);
@@ -378,7 +373,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
         }
         __syncthreads();
     }
-    const float back = minus ? -pow2i(-ex) : pow2i(-ex);
+    const float sign = minus ? -1.f : 1.f;
     if (k.dpart) {
         if (on && open) close_sums((kend + BK - 1) / BK * BK);
         if (zone)
@@ -390,7 +385,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
         const float lo = seq_wave_sum(sum_lo), hi = seq_wave_sum(sum_hi);
         if (lane == 0) { bacc[blo] += lo; bacc[bhi] += hi; }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (head < nh) for (int i = lane; i < nb; i += 64) part_of()[i] = bacc[i] * back;
+        if (head < nh) for (int i = lane; i < nb; i += 64) part_of()[i] = bacc[i] * sign;
     }
     if (!row) return;
     T* dst = reinterpret_cast<T*>(a.dq) + at_row * D;
@@ -401,7 +396,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
         if (c >= D) continue;
         t4 v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = (T)(o[d][j] * (a.scale * back));
+        for (int j = 0; j < 4; ++j) v[j] = (T)(o[d][j] * (a.scale * (sign * down)));
         *reinterpret_cast<t4*>(dst + c) = v;
     }
 }
@@ -423,7 +418,8 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g4 = lane >> 4, li = lane & 15;
     T* tiles = reinterpret_cast<T*>(lds);                                    // QB of Q, 2 of dO
     float* rowv = reinterpret_cast<float*>(tiles + (QB + 2) * BQ * PT);      // of a tile's rows: exponent to add, -D, window index, position; twice
-    float* pass = rowv + 8 * BQ;                                             // pairs: P on its way to the other wave, [2][2 pairs]
+    int* tile_exp = reinterpret_cast<int*>(rowv + 8 * BQ);                   // fp16: exponents of the two tiles of rows
+    float* pass = rowv + 8 * BQ + 4;                                         // pairs: P on its way to the other wave, [2][2 pairs]
     float* tab = pass + (PAIR ? 4 * PW : 0);
     float* window = tab + k.G * a.num_buckets;
 
@@ -446,8 +442,8 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
     int qbeg = 0;                                                            // causal: rows before the first that sees key c0 are skipped
     if (a.causal && c0 > shift) { qbeg = c0 - shift < qr.len ? c0 - shift : qr.len; qbeg -= qbeg % k.qt; }
     const int qfirst = (qr.len + k.qt - 1) / k.qt * k.qt - k.qt;             // from the last rows to the first: the tiles of keys read the same rows at a time
-    const int ex = ds_exponent<T>(k);
-    const float up = pow2i(ex), back = pow2i(-ex);
+    int ex = DS_FREE;                                                        // fp16: dK holds 2^ex of its value
+    float up = pow2i(ex);
     const int role = PAIR ? __builtin_amdgcn_readfirstlane((wave >> 1) ^ (int)(blockIdx.x >> 8 & 1)) : 0, part = PAIR ? wave & 1 : wave;
     v8<T> kf[MK][Dm::KS], vf[PAIR ? 1 : MK][Dm::KS];                         // pairs: kf holds K or V
     int key[MK];
@@ -475,16 +471,22 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
     sq.init_rows((int)a.q_row * (int)sizeof(T), (int)a.q_head * (int)sizeof(T), k.G, k.rt, D, PT);
     sd.init_rows((int)a.do_row * (int)sizeof(T), (int)a.do_head * (int)sizeof(T), k.G, k.rt, D, PT);
     float2 st = {__builtin_inff(), 0.f};
+    int se = DS_FREE;
     const float2* stats = reinterpret_cast<const float2*>(k.delta) + qr.row0 * a.heads + kvh * k.G;
     const int my_qi = (int)threadIdx.x / k.G, my_g = (int)threadIdx.x - my_qi * k.G;       // of the tile's row threadIdx.x
     const long qstep = k.qt * a.q_row, dstep = k.qt * a.do_row, sstep = (long)k.qt * a.heads;
     const T *qp = qb + qfirst * a.q_row, *dp_ = db + qfirst * a.do_row;
     const float2* sp = stats + (long)(qfirst + my_qi) * a.heads + my_g;
+    const int* ep = k.row_exp + (sp - reinterpret_cast<const float2*>(k.delta));
     const auto fetch = [&](int q0) {                                         // the tiles come one after the other
         const int n = qr.len - q0 < k.qt ? (qr.len - q0) * k.G : k.rt;
         sq.fetch_rows(qp, n, PT);
         sd.fetch_rows(dp_, n, PT);
         if (threadIdx.x < BQ) st = (int)threadIdx.x < n ? *sp : float2{__builtin_inff(), 0.f};
+        if constexpr (SCALED<T>) {
+            if (threadIdx.x < BQ) se = (int)threadIdx.x < n ? *ep : DS_FREE;
+            ep -= sstep;
+        }
         qp -= qstep; dp_ -= dstep; sp -= sstep;
     };
     // offsets a tile of rows meets: c0 - phi .. c0 + BKV - 1 - plo
@@ -508,8 +510,26 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
             v[BQ] = -st.y;
             reinterpret_cast<int*>(v)[2 * BQ] = close && pos <= phi ? my_g * k.win - pos - wbeg : -c0;   // + key; rows past the end read word 0 on
             reinterpret_cast<int*>(v)[3 * BQ] = pos;
+            if constexpr (SCALED<T>) {                                       // the smallest over the tile's 32 rows, in lane 31
+                static_assert(BQ == 32, "a half wave holds a tile's rows");
+                int e = se;
+                e = dpp_min<0x111, 0xf>(e); e = dpp_min<0x112, 0xf>(e); e = dpp_min<0x114, 0xf>(e); e = dpp_min<0x118, 0xf>(e);
+                e = dpp_min<0x142, 0x2>(e);
+                if (threadIdx.x == 31) tile_exp[buf] = e;
+            }
         }
     };
+    // fp16: before a tile's dS is added.  Where its rows need a smaller factor, what was added before takes it, too (a power of two: exact).
+    const auto follow = [&](int e) {
+        if (e >= ex) return;
+        const float f = pow2i(e - ex);
+        ex = e; up = pow2i(e);
+#pragma unroll
+        for (int m = 0; m < MK; ++m)
+#pragma unroll
+            for (int d = 0; d < Dm::ND; ++d) dk[m][d] *= f;
+    };
+    const auto exponent_of = [&](int buf) { return SCALED<T> ? __builtin_amdgcn_readfirstlane(tile_exp[buf]) : 0; };
     if (qbeg < qr.len) {
         fetch(qfirst);
         if (a.table) {
@@ -599,7 +619,7 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float d = p[n][m][r] * dp[n][m][r];
-                    if constexpr (__is_same(T, half_t)) d *= up;
+                    if constexpr (SCALED<T>) d *= up;
                     dp[n][m][r] = d;
                 }
     };
@@ -622,7 +642,8 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
         }
     };
     if constexpr (!PAIR) {
-        walk([&](const T* qt, const T* dt, const float* rv, int, int q0) {
+        walk([&](const T* qt, const T* dt, const float* rv, int buf, int q0) {
+            if constexpr (SCALED<T>) follow(exponent_of(buf));
             f32x4 sc[NQ][MK], dp[NQ][MK];
             v8<T> qf[NQ][Dm::KS], df[NQ][Dm::KS];
             read_rows(qt, qf);
@@ -690,8 +711,9 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
     } else {
         f32x4 dp[NQ][MK];
         const T* qlast = tiles;
-        int last = -1;
+        int last = -1, last_exp = DS_FREE;
         const auto key_gradient = [&]() {                                    // dK of the tile before, with the P that the other wave left
+            if constexpr (SCALED<T>) follow(last_exp);
             f32x4 p[NQ][MK];
             const float* from = pass + (last * 2 + part) * PW;
 #pragma unroll
@@ -721,12 +743,14 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
 #pragma unroll
                 for (int m = 0; m < MK; ++m) dp[n][m] = now[n][m];
             qlast = qt; last = buf;
+            last_exp = exponent_of(buf);
         });
         if (last >= 0) key_gradient();
     }
 #pragma unroll
     for (int m = 0; m < MK; ++m) {
         if (key[m] >= kr.len) continue;
+        const float back = SCALED<T> ? pow2i(-ex) : 1.f;
         const long at = ((kr.row0 + key[m]) * a.kv_heads + kvh) * D;
         typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -776,7 +800,7 @@ __global__ __launch_bounds__(1024) void rel_dtable_kernel(const RelAttn k, int w
 // training step, 24 x 12 heads of 64: 660 us with two blocks, 612 with one; causal, heads of 128: 1305, with spills, and 1079).
 constexpr int BK_DQ = 32, BQ_DKV = 32;
 
-struct BwdPlan { int keys, ht, q_rt, q_tiles, k_tiles, n_amax, amax_parts; long rows, units; int64_t stat, amax, part; };
+struct BwdPlan { int keys, ht, q_rt, q_tiles, k_tiles, n_amax; long rows, units; int64_t stat, exps, amax, part; };
 BwdPlan bwd_plan(const cv_rel_attn& a) {
     BwdPlan p;
     const int G = a.heads / a.kv_heads;
@@ -787,14 +811,15 @@ BwdPlan bwd_plan(const cv_rel_attn& a) {
     p.q_tiles = q_parts * ((G + p.ht - 1) / p.ht);
     p.k_tiles = (a.max_k + p.keys - 1) / p.keys;
     p.rows = a.q_off ? a.rows_q : (long)a.n_seq * a.max_q;
-    const long most_q = (long)a.max_q * a.heads, most_k = (long)a.max_k * a.kv_heads;
-    const long blocks = ((most_q > most_k ? most_q : most_k) + 15) / 16, share = a.n_seq > 0 && a.n_seq < 1024 ? 1024 / a.n_seq : 1;        // of a sequence
-    p.amax_parts = (int)(blocks < share ? (blocks < 1 ? 1 : blocks) : share);
-    p.n_amax = (a.n_seq < 1 ? 1 : a.n_seq < 1024 ? a.n_seq : 1024) * p.amax_parts;
+    const bool scaled = a.dtype == CV_DTYPE_F16;
+    const int64_t pairs = (int64_t)a.n_seq * a.kv_heads;                     // parts of a pair: until there are about 1024 workgroups of 64 rows or more
+    const long share = pairs < 1 ? 1 : pairs < 1024 ? 1024 / pairs : 1, runs = (a.max_k + 63L) / 64;
+    p.n_amax = (int)(runs < share ? (runs < 1 ? 1 : runs) : share);
     p.units = (long)a.n_seq * q_parts * (p.q_rt / 16);
     const auto round = [](int64_t n) { return (n + 15) / 16 * 16; };
     p.stat = round(p.rows * a.heads * 8);
-    p.amax = round((int64_t)p.n_amax * 8);
+    p.exps = scaled ? round(p.rows * a.heads * 4) : 0;
+    p.amax = scaled ? round(pairs * p.n_amax * 4) : 0;
     p.part = a.dtable ? round(p.units * a.heads * (int64_t)a.num_buckets * 4) : 0;
     return p;
 }
@@ -806,9 +831,11 @@ int bwd_launch(RelAttn& k, const BwdPlan& p, hipStream_t st) {
     const cv_rel_attn& a = k.a;
     const int G = k.G;
     int rc = 0;
-    if constexpr (__is_same(T, half_t)) {
-        hipLaunchKernelGGL((rel_amax_kernel<T>), dim3(p.n_amax), dim3(256), 0, st, k, p.amax_parts);
-        if ((rc = (int)hipGetLastError())) return rc;
+    if constexpr (SCALED<T>) {
+        if (p.q_tiles > 0 && a.n_seq > 0) {
+            hipLaunchKernelGGL((rel_vnorm_kernel<T>), dim3((unsigned)(a.n_seq * a.kv_heads * p.n_amax)), dim3(256), 0, st, k);
+            if ((rc = (int)hipGetLastError())) return rc;
+        }
     }
     const size_t tabs = a.table ? (size_t)G * a.num_buckets : 0;
     if (p.q_tiles > 0 && a.n_seq > 0) {
@@ -824,7 +851,7 @@ int bwd_launch(RelAttn& k, const BwdPlan& p, hipStream_t st) {
         k.tiles = p.k_tiles; k.rt = BQ_DKV / G * G; k.qt = BQ_DKV / G;
         const auto kernel = &rel_attn_dkv_kernel<T, DT, MK, BQ_DKV, PAIR>;
         k.win = a.table ? window_size(a, G, p.keys + BQ_DKV / G) : 0;
-        const size_t bytes = (PAIR ? 5 : 4) * BQ_DKV * pitch_of<T>(Dims<DT>::W) * sizeof(T) + (8 * BQ_DKV + (PAIR ? 4 * BQ_DKV * 32 : 0) + tabs + (size_t)G * k.win) * 4;
+        const size_t bytes = (PAIR ? 5 : 4) * BQ_DKV * pitch_of<T>(Dims<DT>::W) * sizeof(T) + (8 * BQ_DKV + 4 + (PAIR ? 4 * BQ_DKV * 32 : 0) + tabs + (size_t)G * k.win) * 4;
         if ((rc = allow_lds(kernel, bytes))) return rc;
         hipLaunchKernelGGL(kernel, dim3(part_grid(k)), dim3(256), bytes, st, k);
         if ((rc = (int)hipGetLastError())) return rc;
@@ -854,7 +881,7 @@ int64_t rel_attention_bwd_tiles(const cv_rel_attn& a) {
 }
 int64_t rel_attention_bwd_ws(const cv_rel_attn& a) {
     const BwdPlan p = bwd_plan(a);
-    return p.stat + p.amax + p.part;
+    return p.stat + p.exps + p.amax + p.part + 16;                           // (never 0)
 }
 
 int launch_rel_attention_grad(const cv_rel_attn& a, hipStream_t st) {
@@ -864,8 +891,9 @@ int launch_rel_attention_grad(const cv_rel_attn& a, hipStream_t st) {
     if (!a.table) k.a.num_buckets = 0;
     char* ws = reinterpret_cast<char*>(a.ws);
     k.delta = reinterpret_cast<float*>(ws);
-    k.amax = reinterpret_cast<float*>(ws + p.stat); k.n_amax = p.n_amax;
-    k.dpart = a.dtable ? reinterpret_cast<float*>(ws + p.stat + p.amax) : nullptr;
+    k.row_exp = reinterpret_cast<int*>(ws + p.stat);
+    k.amax = reinterpret_cast<float*>(ws + p.stat + p.exps); k.n_amax = p.n_amax;
+    k.dpart = a.dtable ? reinterpret_cast<float*>(ws + p.stat + p.exps + p.amax) : nullptr;
     k.units = (int)p.units;
     return a.dtype == CV_DTYPE_F16 ? bwd_t<half_t>(k, p, st) : a.dtype == CV_DTYPE_BF16 ? bwd_t<bhalf_t>(k, p, st) : bwd_t<float>(k, p, st);
 }

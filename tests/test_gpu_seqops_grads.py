@@ -127,3 +127,63 @@ def test_gradients_that_fit_their_type_survive_large_and_small_values(dtype, dsc
         want, bound = ref[name]
         assert bool(torch.isfinite(want.to(dtype)).all()) and bool(torch.isfinite(x).all()), name
         assert bool(((x[0].double().cpu() - want).abs() <= bound).all()), name
+
+
+def _rounded_once(want, dtype, terms):
+    """Size of the error of a result that is rounded once and sums rounded dS: `terms` is the root of the sum of squares of what it sums, each rounded by
+    u / sqrt(3) of itself (independent; fp16's own subnormals are in the result's rounding)."""
+    return math.hypot(float((want.to(dtype).double() - want).norm()), R.half_step(dtype) / math.sqrt(3) * float(terms.norm()))
+
+
+def _root_of_squares(q, k, v, do, causal):
+    """One head: dq, dk in 64 bits and, for each element, the root of the sum of the squares of its terms."""
+    q, k, v, do = (x[:, 0].double() for x in (q, k, v, do))
+    s = q @ k.T * q.shape[1] ** -0.5
+    if causal:
+        s = s.masked_fill(torch.arange(len(k))[None] > torch.arange(len(q))[:, None] + len(k) - len(q), -math.inf)
+    p, dp = s.softmax(-1), do @ v.T
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * q.shape[1] ** -0.5
+    return ds @ k, ds.T @ q, (ds.square() @ k.square()).sqrt(), (ds.square().T @ q.square()).sqrt()
+
+
+@HALVES
+@pytest.mark.parametrize("sizes", [(300.0, 3.0, 0.03), (0.03, 300.0, 3.0), (1.0, 1e-2, 1e2)])
+def test_a_sequences_gradients_do_not_hang_on_its_neighbours(dtype, sizes):
+    """Sequences of one call whose dout differ by 1e2 to 1e4, as a loss that is a mean over each sequence's tokens makes them."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(34)
+    lens, dim = (700, 333, 1500), 64
+    mk = lambda n, by=1.0: (torch.randn(n, 1, dim, generator=g) * by).to(dtype)  # noqa: E731
+    parts = [(mk(n), mk(n), mk(n), mk(n, by)) for n, by in zip(lens, sizes)]
+    off = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32).cuda()
+    q, k, v, do = (torch.cat(x).cuda() for x in zip(*parts))
+    saved = ops.rel_attention_train(q, k, v, q_offsets=off, k_offsets=off, max_q=1500, max_k=1500)[1]
+    got = ops.rel_attention_grad(saved, do)
+    at = 0
+    for n, part in zip(lens, parts):
+        dq, dk, tq, tk = _root_of_squares(*part, False)
+        for name, x, want, terms in (("dq", got[0], dq, tq), ("dk", got[1], dk, tk)):
+            off_by = float((x[at:at + n, 0].double().cpu() - want).norm())
+            # of independent errors: their norm strays by 1 / sqrt(2 n), 5 % are allowed for their not being uniform
+            assert off_by <= 1.05 * _rounded_once(want, dtype, terms), (name, n, off_by / _rounded_once(want, dtype, terms))
+        at += n
+
+
+@HALVES
+def test_gradients_of_rows_and_keys_hang_on_their_own_dout(dtype):
+    """Causal, the rows' dout falling by 1e4 along the sequence: the last keys are seen by small rows only."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(35)
+    n, dim = 1024, 64
+    by = 10.0 ** torch.linspace(1.5, -2.5, 8)
+    q, k, v, do = (torch.randn(n, 1, dim, generator=g).to(dtype) for _ in range(4))
+    k, q = (k.float() * 2).to(dtype), (q.float() * 2).to(dtype)
+    do = (do.float() * by.repeat_interleave(n // 8)[:, None, None]).to(dtype)
+    saved = ops.rel_attention_train(q[None].cuda(), k[None].cuda(), v[None].cuda(), causal=True)[1]
+    got = ops.rel_attention_grad(saved, do[None].cuda())
+    dq, dk, tq, tk = _root_of_squares(q, k, v, do, True)
+    for name, x, want, terms in (("dq", got[0], dq, tq), ("dk", got[1], dk, tk)):
+        for i in range(8):
+            part = slice(i * n // 8, (i + 1) * n // 8)
+            off_by = float((x[0, part, 0].double().cpu() - want[part]).norm())
+            assert off_by <= 1.05 * _rounded_once(want[part], dtype, terms[part]), (name, i, off_by / _rounded_once(want[part], dtype, terms[part]))
