@@ -45,6 +45,8 @@ __device__ __forceinline__ int ds_exponent(float b2) {
     return 14 - (((int)(__float_as_uint(b2) >> 23) - 127) >> 1);             // -50 for infinities
 }
 template <typename T> constexpr bool SCALED = __is_same(T, half_t);
+// fp16's P for dV rides on 2^14: P <= 1, and beside 1e5 keys most of it would be subnormal (1.4e-3 of dV at 131072 keys).  It is added to the exponent.
+template <typename T> constexpr int P_UP = SCALED<T> ? 14 : 0;
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
 
 // waves a SIMD to leave registers for: fp32 fragments of wide heads need more than half of them
@@ -443,7 +445,7 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
     if (a.causal && c0 > shift) { qbeg = c0 - shift < qr.len ? c0 - shift : qr.len; qbeg -= qbeg % k.qt; }
     const int qfirst = (qr.len + k.qt - 1) / k.qt * k.qt - k.qt;             // from the last rows to the first: the tiles of keys read the same rows at a time
     int ex = DS_FREE;                                                        // fp16: dK holds 2^ex of its value
-    float up = pow2i(ex);
+    float up = pow2i(ex - P_UP<T>);                                          // from P 2^P_UP (dP - D)
     const int role = PAIR ? __builtin_amdgcn_readfirstlane((wave >> 1) ^ (int)(blockIdx.x >> 8 & 1)) : 0, part = PAIR ? wave & 1 : wave;
     v8<T> kf[MK][Dm::KS], vf[PAIR ? 1 : MK][Dm::KS];                         // pairs: kf holds K or V
     int key[MK];
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
         if (threadIdx.x < BQ) {
             const int pos = plo + my_qi;
             float* v = rowv + buf * 4 * BQ + threadIdx.x;
-            v[0] = (close || !a.table ? 0.f : c0 >= phi ? far_hi : far_lo) - st.x;
+            v[0] = (close || !a.table ? 0.f : c0 >= phi ? far_hi : far_lo) - (st.x - (float)P_UP<T>);
             v[BQ] = -st.y;
             reinterpret_cast<int*>(v)[2 * BQ] = close && pos <= phi ? my_g * k.win - pos - wbeg : -c0;   // + key; rows past the end read word 0 on
             reinterpret_cast<int*>(v)[3 * BQ] = pos;
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
     const auto follow = [&](int e) {
         if (e >= ex) return;
         const float f = pow2i(e - ex);
-        ex = e; up = pow2i(e);
+        ex = e; up = pow2i(e - P_UP<T>);
 #pragma unroll
         for (int m = 0; m < MK; ++m)
 #pragma unroll
@@ -590,7 +592,7 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
 #pragma unroll
                 for (int m = 0; m < MK; ++m) acc[n][m] = Seq<T>::mma(rows[n][ks], keys[m][ks], acc[n][m]);
     };
-    const auto weights = [&](const float* rv, int q0, f32x4 (&sc)[NQ][MK]) {            // S -> P
+    const auto weights = [&](const float* rv, int q0, f32x4 (&sc)[NQ][MK]) {            // S -> P 2^P_UP
         if (a.causal && clast > q0 + shift) {
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
@@ -759,13 +761,13 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
             if (c >= D) continue;
             t4 x, y;
             if constexpr (PAIR) {
-                const float f = role ? a.scale * back : 1.f;
+                const float f = role ? a.scale * back : pow2i(-P_UP<T>);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = (T)(dk[m][d][j] * f);
                 *reinterpret_cast<t4*>(reinterpret_cast<T*>(role ? a.dk : a.dv) + at + c) = x;
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { x[j] = (T)(dk[m][d][j] * (a.scale * back)); y[j] = (T)dv[m][d][j]; }
+                for (int j = 0; j < 4; ++j) { x[j] = (T)(dk[m][d][j] * (a.scale * back)); y[j] = (T)(SCALED<T> ? dv[m][d][j] * pow2i(-P_UP<T>) : dv[m][d][j]); }
                 *reinterpret_cast<t4*>(reinterpret_cast<T*>(a.dk) + at + c) = x;
                 *reinterpret_cast<t4*>(reinterpret_cast<T*>(a.dv) + at + c) = y;
             }

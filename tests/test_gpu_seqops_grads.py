@@ -187,3 +187,20 @@ def test_gradients_of_rows_and_keys_hang_on_their_own_dout(dtype):
             part = slice(i * n // 8, (i + 1) * n // 8)
             off_by = float((x[0, part, 0].double().cpu() - want[part]).norm())
             assert off_by <= 1.05 * _rounded_once(want[part], dtype, terms[part]), (name, i, off_by / _rounded_once(want[part], dtype, terms[part]))
+
+
+@HALVES
+@pytest.mark.parametrize("lk,dim", [(4096, 128), (32768, 64), (131072, 64)])
+def test_gradients_of_values_among_many_keys(dtype, lk, dim):
+    ops = _ops()
+    g = torch.Generator().manual_seed(36)
+    lq = 48
+    q, k, v, do = (torch.randn(n, 1, dim, generator=g).to(dtype) for n in (lq, lk, lk, lq))
+    do = (do.float() * lk / 64).to(dtype)                                    # gradients of normal size
+    saved = ops.rel_attention_train(q[None].cuda(), k[None].cuda(), v[None].cuda())[1]
+    got = ops.rel_attention_grad(saved, do[None].cuda())[2][0, :, 0].double().cpu()
+    qd, kd, dd = (x[:, 0].double() for x in (q, k, do))
+    p = (qd @ kd.T * dim ** -0.5).softmax(-1)
+    want, terms = p.T @ dd, (p.T.square() @ dd.square()).sqrt()
+    off_by, size = float((got - want).norm()), _rounded_once(want, dtype, terms)
+    assert off_by <= 1.05 * size, off_by / size
