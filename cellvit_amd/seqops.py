@@ -4,8 +4,8 @@ For models over the token rows this package hands out: tile tokens ``[B, L, ...]
 (``postproc.pool_cell_tokens``).  Every function runs the HIP kernels of ``libcellvit_amd.so`` on the tensors' device and its current stream; there is
 no CPU fallback.  Nothing synchronises; every call can be captured into a graph, but for those that autograd records.
 
-``rel_bias``, ``rel_attention`` and ``block_norm`` are differentiable (once) through torch's autograd; ``*_train`` / ``*_grad`` are the two
-halves by themselves, for programs that keep their own backward pass or capture it.
+``rel_bias``, ``rel_attention`` and ``block_norm`` are differentiable (once, backward; forward-mode tangents are refused) through torch's autograd;
+``*_train`` / ``*_grad`` are the two halves by themselves, for programs that keep their own backward pass or capture it.
 """
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 
@@ -57,9 +58,19 @@ def _call(device: int, fn, *args) -> None:
         _lib.check(rc)
 
 
+def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors that carry a forward-mode derivative: the kernels know none and would drop it."""
+    if _forward_ad._current_level < 0:                       # no level is open: nothing carries one
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the sequence operators have no forward-mode derivatives")
+
+
 def _differentiable(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether autograd is to record the call.  Not inside a graph capture: torch adds a leaf's gradients on the stream where the leaf was first
     used, and a captured backward pass that meets an eager graph's addition on another stream ends the process."""
+    _no_tangents(*tensors)
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
         return False
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
@@ -144,6 +155,7 @@ def rel_bias(table: torch.Tensor, buckets: torch.Tensor, q_len: int, k_len: int,
 def rel_bias_grad(dbias: torch.Tensor, buckets: torch.Tensor, num_buckets: int, *, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Gradient of the table, [num_buckets, heads] of ``dtype`` (float32 or dbias' own), from ``dbias`` [heads, q_len, k_len] or, where a batch
     shares the plane, [batch, heads, q_len, k_len]."""
+    _no_tangents(dbias)
     span = _check_map(buckets)
     if dbias.dim() not in (3, 4):
         raise ValueError("dbias must be [heads, q_len, k_len] or [batch, heads, q_len, k_len]")
@@ -335,6 +347,7 @@ def rel_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: Opti
 def rel_attention_train(q, k, v, table=None, buckets=None, *, scale=None, causal=False, q_offsets=None, k_offsets=None, max_q=None, max_k=None
                         ) -> Tuple[torch.Tensor, RelAttentionSaved]:
     """``rel_attention`` that also returns what its backward pass reads (the inputs are kept, not copied)."""
+    _no_tangents(q, k, v, table)
     c = _attn_setup(q, k, v, table, buckets, scale, causal, q_offsets, k_offsets, max_q, max_k, 1)
     out, lse, lo = _attn_forward(c, None, True)
     return out, RelAttentionSaved(*c[1:8], out, lse, lo, *c[8:12])
@@ -344,6 +357,7 @@ def rel_attention_grad(saved: RelAttentionSaved, dout: torch.Tensor, *, table_gr
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """(dq, dk, dv, dtable) of ``rel_attention``, each of its input's dtype; dtable None without a table or with ``table_grad`` false."""
     s = saved
+    _no_tangents(s.q, s.k, s.v, s.table, dout)
     if dout.shape != s.out.shape or dout.dtype != s.out.dtype:
         raise ValueError(f"dout must be {s.out.dtype} {list(s.out.shape)}")
     c = _attn_setup(s.q, s.k, s.v, s.table, s.buckets, s.scale, s.causal, s.q_offsets, s.k_offsets, s.max_q, s.max_k, 1)
@@ -479,6 +493,7 @@ def block_norm(x: torch.Tensor, y: torch.Tensor, *, post=None, pre=None, gate: O
 
 def block_norm_train(x, y, *, post=None, pre=None, gate=None, rows_per_gate=None, alpha=1.0, kind="layer", eps=1e-6):
     """``block_norm`` that also returns what its backward pass reads (y is kept, not copied)."""
+    _no_tangents(x, y, gate, *(post if isinstance(post, (tuple, list)) else (post,)), *(pre if isinstance(pre, (tuple, list)) else (pre,)))
     return _block_norm(x, y, post, pre, gate, rows_per_gate, alpha, kind, eps, True)
 
 
@@ -486,6 +501,7 @@ def block_norm_grad(saved: BlockNormSaved, dx_out: Optional[torch.Tensor], dz: O
     """Gradients {dx, dy, post_w, post_b, gate, pre_w, pre_b} from those of x_out and z (either may be None); weights and gate float32, None where the
     forward had none.  dx and dy are [rows, C]."""
     s = saved
+    _no_tangents(s.y, s.x_out, s.gate, *(s.post or ()), *(s.pre or ()), dx_out, dz)
     m, width = s.y.shape
     dev = s.y.device
     if dz is not None:

@@ -37,3 +37,28 @@ def test_python_raises_what_the_workspace_size_refuses(monkeypatch):
             fn(q, k, k)
     with pytest.raises(NotImplementedError, match="head_dim"):
         seqops.rel_attention(q[:, :, :1, :60], k[..., :60], k[..., :60])
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tensors_that_carry_a_forward_mode_tangent_are_refused(grad):
+    """The kernels would return a tensor without one, as if the derivative were zero."""
+    import torch.autograd.forward_ad as fwd
+    t = torch.zeros
+    m = seqops.rel_buckets(8, 16, True, device="cpu")
+    q, table, x, w = t(1, 5, 2, 16), t(8, 2), t(6, 32), t(32)
+    saved = seqops.RelAttentionSaved(q, q, q, table, m, None, None, q, t(1, 5, 2), None, 0.25, False, 5, 5)
+    kept = seqops.BlockNormSaved(x, x, t(6, 4), None, (w, None), None, 6, 1.0, "layer", 1e-6)
+    with fwd.dual_level():
+        d = lambda p: fwd.make_dual(p.clone().requires_grad_(grad), torch.ones_like(p))  # noqa: E731
+        calls = [lambda: seqops.rel_bias(d(table), m, 3, 3), lambda: seqops.rel_bias_grad(d(t(2, 3, 3)), m, 8), lambda: seqops.rel_attention(d(q), q, q),
+                 lambda: seqops.rel_attention(q, q, d(q)), lambda: seqops.rel_attention(q, q, q, d(table), m), lambda: seqops.rel_attention_train(q, d(q), q),
+                 lambda: seqops.rel_attention_grad(saved, d(q)), lambda: seqops.rel_attention_grad(saved._replace(v=d(q)), q), lambda: seqops.block_norm(d(x), x, pre=w),
+                 lambda: seqops.block_norm(x, d(x), pre=w), lambda: seqops.block_norm(x, x, post=(w, d(w))), lambda: seqops.block_norm(x, x, gate=d(w)),
+                 lambda: seqops.block_norm_train(x, x, pre=d(w)), lambda: seqops.block_norm_grad(kept, d(x), None), lambda: seqops.block_norm_grad(kept, x, d(x))]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU fallback"):                             # a level alone changes nothing
+            seqops.rel_attention(q, q, q)
