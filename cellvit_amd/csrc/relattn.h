@@ -243,6 +243,7 @@ template <typename F> inline int allow_lds(F* kernel, size_t bytes) {
 }
 
 int64_t rel_attention_bwd_tiles(const cv_rel_attn& a);
+int launch_rel_zero(void* base, int dtype, long rows, int heads, int D, long row, long head, hipStream_t st);
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }

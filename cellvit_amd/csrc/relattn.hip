@@ -623,6 +623,24 @@ template <typename T> int fwd_t(RelAttn& k, int mq, hipStream_t st) {
 
 }  // namespace
 
+// Rows of `heads` heads that no sequence owns because there are no sequences, or none of any length, so that no kernel starts that would zero them.  Moves
+// 16 bytes a thread a turn.
+__global__ __launch_bounds__(256) void rel_zero_kernel(char* base, long pieces, int per_row, int per_head, long row, long head) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (long)gridDim.x * 256) {
+        const long t = i / per_row;
+        const int c = (int)(i - t * per_row), h = c / per_head;
+        *reinterpret_cast<u32x4*>(base + t * row + h * head + (c - h * per_head) * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
+}
+int launch_rel_zero(void* base, int dtype, long rows, int heads, int D, long row, long head, hipStream_t st) {
+    if (!base || rows <= 0) return 0;
+    const int es = dtype == CV_DTYPE_F32 ? 4 : 2, per_head = D * es / 16;
+    const long pieces = rows * heads * per_head, groups = (pieces + 255) / 256;
+    hipLaunchKernelGGL(rel_zero_kernel, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, reinterpret_cast<char*>(base), pieces, heads * per_head, per_head, row * es,
+                       head * es);
+    return (int)hipGetLastError();
+}
+
 static bool keeps_rest(const cv_rel_attn& a) { return a.out_lo && a.dtype != CV_DTYPE_F32; }
 
 int64_t rel_attention_tiles(const cv_rel_attn& a, bool grad) {
@@ -639,7 +657,7 @@ int64_t rel_attention_fwd_ws(const cv_rel_attn& a) {
 }
 
 int launch_rel_attention(const cv_rel_attn& a, hipStream_t st) {
-    if (a.n_seq == 0 || a.max_q == 0) return 0;
+    if (a.n_seq == 0 || a.max_q == 0) return a.zero_rest && a.q_off ? launch_rel_zero(a.out, a.dtype, a.rows_q, a.heads, a.head_dim, a.o_row, a.o_head, st) : 0;
     const FwdPlan p = fwd_plan(a);
     RelAttn k{};
     k.a = a; k.G = a.heads / a.kv_heads; k.rt = p.rt; k.qt = p.rt / k.G; k.tiles = p.tiles; k.nsplit = p.nsplit; k.split_tiles = p.split_tiles;

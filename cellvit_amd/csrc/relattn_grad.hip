@@ -3,6 +3,8 @@
 // Two kernels that each own what they write (dQ and the table's gradient by rows, dK and dV by keys), so no sum depends on scheduling; the price is
 // seven products where five would do.
 // fp16: a row's dS is scaled by a power of two from |dO_i| and max |V_j| for the products (exact, taken out of the results): ds_exponent.
+#include <initializer_list>
+
 #include "relattn.h"
 
 namespace cva {
@@ -888,6 +890,12 @@ int64_t rel_attention_bwd_ws(const cv_rel_attn& a) {
 
 int launch_rel_attention_grad(const cv_rel_attn& a, hipStream_t st) {
     const BwdPlan p = bwd_plan(a);
+    const long D = a.head_dim;
+    int rc = 0;
+    if (a.zero_rest && a.q_off && (a.n_seq == 0 || a.max_q == 0) && (rc = launch_rel_zero(a.dq, a.dtype, a.rows_q, a.heads, a.head_dim, a.heads * D, D, st))) return rc;
+    if (a.zero_rest && a.k_off && (a.n_seq == 0 || a.max_k == 0))
+        for (void* t : {a.dk, a.dv})
+            if ((rc = launch_rel_zero(t, a.dtype, a.rows_k, a.kv_heads, a.head_dim, a.kv_heads * D, D, st))) return rc;
     RelAttn k{};
     k.a = a; k.G = a.heads / a.kv_heads; k.nsplit = 1; k.c = a.scale * LOG2E;
     if (!a.table) k.a.num_buckets = 0;

@@ -296,7 +296,7 @@ def _attn_call(c: _Attn, grad: int, strides: tuple, ptrs: tuple) -> None:
 def _attn_forward(c: _Attn, out, train):
     q = c.q
     if out is None:                                          # zero_rest: the kernels zero the rows that no sequence owns
-        out = (torch.empty_like if c.n_seq and c.max_q else torch.zeros_like)(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     so = _rows(out, 1)[1]
     lse = torch.empty(q.shape[:-1], dtype=_F32, device=q.device) if train else None
     lo = torch.empty(q.shape, dtype=_F32, device=q.device) if train and q.dtype is not _F32 else None
@@ -364,9 +364,7 @@ def rel_attention_grad(saved: RelAttentionSaved, dout: torch.Tensor, *, table_gr
     _same_device(s.q, dout)
     dout, sd = _rows(dout, 16 // dout.element_size())
     flat = torch.contiguous_format
-    dq = (torch.empty_like if c.n_seq and c.max_q else torch.zeros_like)(s.q, memory_format=flat)
-    new = torch.empty_like if c.n_seq and c.max_k else torch.zeros_like
-    dk, dv = new(s.k, memory_format=flat), new(s.k, memory_format=flat)
+    dq, dk, dv = (torch.empty_like(t, memory_format=flat) for t in (s.q, s.k, s.k))
     dtable = torch.empty_like(s.table, memory_format=flat) if s.table is not None and table_grad else None
     _attn_call(c, 1, (*_rows(s.out, 1)[1], *sd),
                (s.out.data_ptr(), s.lse.data_ptr(), _ptr(s.out_lo), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable)))

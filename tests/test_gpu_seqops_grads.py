@@ -1,12 +1,13 @@
 """GPU: gradients of the sequence operators held to what their types allow, each entry's errors added as independent ones (the bounds of test_gpu_seqops.py
 add the worst of every pair)."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 import seq_ref as R
-from test_gpu_seqops import BF16, F16, _map, _ops, _pack
+from test_gpu_seqops import BF16, F16, F32, TYPES, _map, _ops, _pack
 
 pytestmark = pytest.mark.gpu
 HALVES = pytest.mark.parametrize("dtype", [F16, BF16])
@@ -204,3 +205,30 @@ def test_gradients_of_values_among_many_keys(dtype, lk, dim):
     want, terms = p.T @ dd, (p.T.square() @ dd.square()).sqrt()
     off_by, size = float((got - want).norm()), _rounded_once(want, dtype, terms)
     assert off_by <= 1.05 * size, off_by / size
+
+
+@TYPES
+def test_rows_of_no_sequence_are_zeroed_where_there_is_nothing_to_attend_to(dtype):
+    """No sequences, or none of any length: packed rows belong to nobody and get zeros from the C entries, too (zero_rest), or stay as they were."""
+    from cellvit_amd import _lib
+    lib, code = _lib.load(), {F16: _lib.DTYPE_F16, BF16: _lib.DTYPE_BF16, F32: _lib.DTYPE_F32}[dtype]
+    T, H, D = 37, 3, 24
+    for n_seq, most_q, most_k in ((0, 5, 5), (2, 0, 5), (2, 5, 0)):
+        off = torch.full((n_seq + 1,), 10, dtype=torch.int32, device="cuda")
+        q, do = (torch.randn(T, H, D, device="cuda").to(dtype) for _ in range(2))
+        for zero in (0, 1):
+            out = torch.full((T, 2 * H, D), 7.0, dtype=dtype, device="cuda")[:, H:]           # strided: every second block of heads
+            grads = [torch.full((T, H, D), 7.0, dtype=dtype, device="cuda") for _ in range(3)]
+            lse, ws = torch.zeros(T, H, device="cuda"), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+            a = _lib.cv_rel_attn(dtype=code, n_seq=n_seq, heads=H, kv_heads=H, head_dim=D, max_q=most_q, max_k=most_k, scale=0.2, zero_rest=zero, rows_q=T, rows_k=T, q_row=H * D,
+                                 q_head=D, k_row=H * D, k_head=D, v_row=H * D, v_head=D, o_row=2 * H * D, o_head=D, do_row=H * D, do_head=D, q=q.data_ptr(), k=q.data_ptr(),
+                                 v=q.data_ptr(), q_off=off.data_ptr(), k_off=off.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(), dout=do.data_ptr(), dq=grads[0].data_ptr(),
+                                 dk=grads[1].data_ptr(), dv=grads[2].data_ptr(), ws=ws.data_ptr(), ws_bytes=ws.numel())
+            for fn in (lib.cv_op_rel_attention, lib.cv_op_rel_attention_grad):
+                _lib.check(fn(C.byref(a), torch.cuda.current_stream().cuda_stream))
+            want = 0.0 if zero else 7.0
+            for t in (out, *grads):
+                assert bool((t == want).all()), (n_seq, most_q, most_k, zero)
+            assert bool((out._base[:, :H] == 7).all())
+        got = _ops().rel_attention(q, q, q, q_offsets=off, k_offsets=off, max_q=most_q, max_k=most_k)
+        assert not got.any()
