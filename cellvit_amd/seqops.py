@@ -28,6 +28,18 @@ _ATTN, _NORM = struct.Struct("@10if3i17q16Pq"), struct.Struct("@6i2f6q20Pq")
 assert _ATTN.size == C.sizeof(_lib.cv_rel_attn) and _NORM.size == C.sizeof(_lib.cv_block_norm)
 
 
+def _pack(layout: struct.Struct, *fields) -> bytes:
+    try:
+        return layout.pack(*fields)
+    except struct.error as e:                                # a size beyond the C struct's 32 bits
+        raise ValueError(f"a size or length is out of range ({e})") from None
+
+
+def _plane_sizes(q_len: int, k_len: int) -> None:
+    if not (0 <= q_len <= 1 << 22 and 0 <= k_len <= 1 << 22):
+        raise ValueError(f"a bias plane has 0 to 2^22 rows and columns (got {q_len}, {k_len})")
+
+
 def _dtype(t: torch.dtype) -> int:
     code = _DTYPES.get(t)
     if code is None:
@@ -116,11 +128,12 @@ def _check_table(table: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 def _rel_bias(table, buckets, q_len, k_len, dtype, out):
     span = _check_map(buckets)
+    _plane_sizes(q_len, k_len)
     dtype = out.dtype if out is not None and dtype is None else dtype or table.dtype
     table = _check_table(table, dtype)
     nb, heads = table.shape
     if out is None:
-        out = torch.empty((heads, max(q_len, 0), max(k_len, 0)), dtype=dtype, device=table.device)
+        out = torch.empty((heads, q_len, k_len), dtype=dtype, device=table.device)
     elif tuple(out.shape) != (heads, q_len, k_len) or not out.is_contiguous() or out.dtype != dtype:
         raise ValueError(f"out must be contiguous [{heads}, {q_len}, {k_len}]")
     code = _dtype(out.dtype)
@@ -166,6 +179,9 @@ def rel_bias_grad(dbias: torch.Tensor, buckets: torch.Tensor, num_buckets: int, 
     dbias = dbias.contiguous()
     batch = dbias.shape[0] if dbias.dim() == 4 else 1
     heads, q_len, k_len = dbias.shape[-3:]
+    _plane_sizes(q_len, k_len)
+    if not 1 <= num_buckets <= 256 or batch > 0x7fffffff:
+        raise ValueError(f"1 to 256 buckets and less than 2^31 planes (got {num_buckets}, {batch})")
     lib = _lib.load()
     need = lib.cv_op_rel_bias_grad_ws(num_buckets, heads, q_len, k_len)
     if need < 0:
@@ -228,6 +244,8 @@ def _offsets(off: Optional[torch.Tensor], shape, most: Optional[int], name: str)
         raise ValueError(f"offsets of {name} must be an integer vector [sequences + 1]")
     if most is None:
         raise ValueError(f"packed {name} needs the longest length (max_q / max_k)")
+    if shape[0] > 0x7fffffff:
+        raise NotImplementedError(f"packed {name} has more than 2^31 - 1 rows: offsets are int32")
     return off.to(torch.int32).contiguous(), off.numel() - 1, int(most)
 
 
@@ -283,7 +301,7 @@ def _attn_setup(q, k, v, table, buckets, scale, causal, q_offsets, k_offsets, ma
 def _attn_call(c: _Attn, grad: int, strides: tuple, ptrs: tuple) -> None:
     """The C call, with its workspace (which lives until the call returns; the allocator orders its reuse on the stream)."""
     lib = _lib.load()
-    a = _ATTN.pack(*c.head, *strides, *c.tail, *ptrs, 0, 0)
+    a = _pack(_ATTN, *c.head, *strides, *c.tail, *ptrs, 0, 0)
     need = lib.cv_op_rel_attention_ws(a, grad)
     if need < 0:
         _lib.check(-need)
@@ -422,7 +440,7 @@ def _norm_setup(x, y, post, pre, gate, rows_per_gate, kind):
     per = m if rows_per_gate is None else int(rows_per_gate)
     if rows_per_gate is not None and per < 1:
         raise ValueError("rows_per_gate must be positive")
-    per = max(per, 1)
+    per = max(min(per, m), 1)                                # more rows to a group than there are: one group
     if gate is not None:
         groups = max(1, -(-m // per))
         if gate.dtype is not _F32 or gate.numel() != groups * width or gate.shape[-1] != width:
@@ -444,7 +462,7 @@ def _block_norm(x, y, post, pre, gate, rows_per_gate, alpha, kind, eps, train):
     pw, pb = post or (None, None)
     nw, nb = pre or (None, None)
     alpha, eps = float(alpha), float(eps)
-    a = _NORM.pack(code, _KINDS[kind], 0 if post is None else 1, m, width, per, alpha, eps, _row(x), _row(y), width, width, 0, 0, x.data_ptr(), y.data_ptr(),
+    a = _pack(_NORM, code, _KINDS[kind], 0 if post is None else 1, m, width, per, alpha, eps, _row(x), _row(y), width, width, 0, 0, x.data_ptr(), y.data_ptr(),
                    _ptr(pw), _ptr(pb), _ptr(gate), _ptr(nw), _ptr(nb), x_out.data_ptr(), _ptr(z), _ptr(stats), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     _call(device, _lib.load().cv_op_block_norm, a)
     saved = BlockNormSaved(y, x_out, stats, post, pre, gate, per, alpha, kind, eps) if train else None
@@ -521,7 +539,7 @@ def block_norm_grad(saved: BlockNormSaved, dx_out: Optional[torch.Tensor], dz: O
             _row(dz), 0, s.y.data_ptr(), _ptr(pw), _ptr(pb), _ptr(s.gate), _ptr(nw), _ptr(nb), s.x_out.data_ptr(), 0, s.stats.data_ptr(), _ptr(dx_out),
             _ptr(dz), dx.data_ptr(), dy.data_ptr(), _ptr(grads[0]), _ptr(grads[1]), _ptr(dgate), _ptr(grads[2]), _ptr(grads[3]))
     lib = _lib.load()
-    need = lib.cv_op_block_norm_grad_ws(_NORM.pack(*args, 0, 0))
+    need = lib.cv_op_block_norm_grad_ws(_pack(_NORM, *args, 0, 0))
     if need < 0:
         _lib.check(_lib.CV_ERR_INVALID)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)

@@ -62,3 +62,30 @@ def test_tensors_that_carry_a_forward_mode_tangent_are_refused(grad):
                 call()
         with pytest.raises(RuntimeError, match="no CPU fallback"):                             # a level alone changes nothing
             seqops.rel_attention(q, q, q)
+
+
+def test_sizes_beyond_32_bits_are_refused_and_wide_gate_groups_are_one_group(monkeypatch):
+    """None of them may reach the library with its upper bits cut off."""
+    t = torch.zeros
+    m = seqops.rel_buckets(8, 16, True, device="cpu")
+    monkeypatch.setattr(seqops, "_same_device", lambda *a: 0)
+    calls = []
+    monkeypatch.setattr(seqops, "_call", lambda device, fn, a, *rest: calls.append(a))
+    q, off, x = t(7, 2, 16), torch.tensor([0, 7], dtype=torch.int32), t(6, 32)
+    for lq, lk in ((1 << 31, 7), (7, 1 << 40), (-1 << 40, 7), ((1 << 32) + 7, 7)):
+        with pytest.raises(ValueError):
+            seqops.rel_attention(q, q, q, q_offsets=off, k_offsets=off, max_q=lq, max_k=lk)
+    for lq, lk in (((1 << 32) + 3, 3), (3, (1 << 32) + 3), (-1, 3), (3, 1 << 23)):
+        with pytest.raises(ValueError):
+            seqops.rel_bias(t(8, 2), m, lq, lk)
+    for nb in (0, 257, (1 << 32) + 8):
+        with pytest.raises(ValueError):
+            seqops.rel_bias_grad(t(2, 3, 3), m, nb)
+    with pytest.raises(NotImplementedError):
+        seqops.rel_attention(q[:1].expand(1 << 31, 2, 16), q, q, q_offsets=off, k_offsets=off, max_q=7, max_k=7)
+    with pytest.raises(ValueError):
+        seqops.block_norm(x, x, gate=t(2, 32), rows_per_gate=1 << 40)      # one group, not two
+    assert not calls
+    for per in (6, 7, 1 << 31, 1 << 40):
+        seqops.block_norm(x, x, gate=t(1, 32), rows_per_gate=per)
+    assert len(calls) == 4 and len({a[:24] for a in calls}) == 1               # the head of the struct: sizes and rows a group
