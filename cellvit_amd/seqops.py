@@ -348,9 +348,10 @@ def rel_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: Opti
 
     q [S, Lq, heads, D], k and v [S, Lk, kv_heads, D] of one dtype (any strides; heads a multiple of kv_heads), or packed rows [T, heads, D] with int32
     ``q_offsets`` / ``k_offsets`` [S + 1] and the longest lengths ``max_q`` / ``max_k``.  Query i of a sequence stands at position
-    i + Lk - Lq; ``causal`` hides later keys.  ``scale`` defaults to D ** -0.5.  A row that sees no key gets zeros.  Rows outside every
-    sequence may hold anything, and are left as they were in ``out`` (zeros without it); keys and values inside one must be finite, hidden ones
-    too.  Strides: rows up to 16 MiB apart, the heads that share a key head up to 1 GiB."""
+    i + Lk - Lq; ``causal`` hides later keys.  ``scale`` (1e-6 to 1e6) defaults to D ** -0.5.  A row that sees no key gets zeros.  Rows outside every
+    sequence may hold anything, and are left as they were in ``out`` (zeros without it; it overlaps no input); keys and values inside one must be finite,
+    hidden ones too.  A table entry of -inf hides its keys; finite ones act as if held to +-1.6e7 / log2(e), beyond which fp32 would lose the scores
+    beside them: two mask levels below that (-1e8, -1e9) are one.  Strides: rows up to 16 MiB apart, the heads that share a key head up to 1 GiB."""
     if _differentiable(q, k, v, table):
         if out is not None:
             raise ValueError("out= is not differentiable: call under torch.no_grad()")
