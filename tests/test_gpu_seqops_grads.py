@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import seq_ref as R
-from test_gpu_seqops import BF16, F16, F32, TYPES, _map, _ops, _pack
+from test_gpu_seqops import BF16, F16, F32, TYPES, _close, _map, _ops, _pack
 
 pytestmark = pytest.mark.gpu
 HALVES = pytest.mark.parametrize("dtype", [F16, BF16])
@@ -232,3 +232,75 @@ def test_rows_of_no_sequence_are_zeroed_where_there_is_nothing_to_attend_to(dtyp
             assert bool((out._base[:, :H] == 7).all())
         got = _ops().rel_attention(q, q, q, q_offsets=off, k_offsets=off, max_q=most_q, max_k=most_k)
         assert not got.any()
+
+
+@TYPES
+@pytest.mark.parametrize("packed_q", [False, True])
+def test_one_side_packed_and_the_other_dense(dtype, packed_q):
+    """Single tokens or a few rows a sequence beside packed keys of any length, and the other way round."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(37)
+    long, short = [0, 1, 700, 63], 3
+    lq, lk = (long, [short] * 4) if packed_q else ([short] * 4, long)
+    mk = lambda n, h: [torch.randn(x, h, 64, generator=g).to(dtype) for x in n]  # noqa: E731
+    qs, ks, vs, dos = mk(lq, 4), mk(lk, 2), mk(lk, 2), mk(lq, 4)
+    table, m = torch.randn(16, 4, generator=g), _map(16, 20, True)
+    off = torch.tensor([0, *torch.tensor(long).cumsum(0).tolist()])                            # 64-bit offsets are taken, too
+    join = lambda x, packed: (torch.cat if packed else torch.stack)(x).cuda()  # noqa: E731
+    kw = dict(q_offsets=off.cuda(), max_q=700) if packed_q else dict(k_offsets=off.cuda(), max_k=700)
+    q, do, k, v = join(qs, packed_q), join(dos, packed_q), join(ks, not packed_q), join(vs, not packed_q)
+    out, saved = ops.rel_attention_train(q, k, v, table.cuda(), m.cuda(), **kw)
+    assert torch.equal(out, ops.rel_attention(q, k, v, table.cuda(), m.cuda(), **kw))
+    dq, dk, dv, dt = ops.rel_attention_grad(saved, do)
+    part = lambda x, i, packed: x[off[i]:off[i + 1]] if packed else x[i]  # noqa: E731
+    refs = [R.attention(*x, table, m, 0.125, False, d) for *x, d in zip(qs, ks, vs, dos)]
+    for i, r in enumerate(refs):
+        for name, x, p in (("out", out, packed_q), ("dq", dq, packed_q), ("dk", dk, not packed_q), ("dv", dv, not packed_q)):
+            _close(part(x, i, p), *r[name], name)
+    _close(dt, sum(r["dtable"][0] for r in refs), sum(r["dtable"][1] for r in refs), "dtable")
+
+
+@HALVES
+@pytest.mark.parametrize("lens,heads,kv,dim", [((2, 600), 16, 2, 128), ((90, 90), 32, 1, 128), ((150, 700), 6, 2, 80)])
+def test_training_halves_whose_first_call_is_captured(dtype, lens, heads, kv, dim):
+    """Kernels that ask for more than 64 KB of LDS, workspaces and all, inside a capture; replays with other inputs and eager work between."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(38)
+    fresh = lambda: [torch.randn(1, n, h, dim, generator=g).to(dtype).cuda() for n, h in zip((lens[0], lens[1], lens[1], lens[0]), (heads, kv, kv, heads))]  # noqa: E731
+    table, m = torch.randn(256, heads, generator=g).cuda(), _map(256, 300, False).cuda()
+
+    def step(q, k, v, do):
+        out, saved = ops.rel_attention_train(q, k, v, table, m, causal=True)
+        return [out, saved.lse, saved.out_lo, *ops.rel_attention_grad(saved, do)]
+    state = fresh()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(*state)
+    for scale in (1.0, 1e-3, 300.0):
+        new = fresh()
+        new[3] *= scale
+        for a, b in zip(state, new):
+            a.copy_(b)
+        graph.replay()
+        got = [t.clone() for t in held]
+        want = step(*new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@HALVES
+def test_autograd_with_a_float32_table_equals_the_halves(dtype):
+    ops = _ops()
+    g = torch.Generator().manual_seed(39)
+    q, k, v = (torch.randn(2, 130, 3, 64, generator=g).to(dtype).cuda().requires_grad_(True) for _ in range(3))
+    table, m = torch.randn(3, 32, generator=g).cuda().T.requires_grad_(True), _map(32, 50, True).cuda()      # [buckets, heads], not contiguous
+    do = torch.randn(2, 130, 3, 64, generator=g).to(dtype).cuda()
+    out = ops.rel_attention(q, k, v, table, m)
+    got = torch.autograd.grad(out, (q, k, v, table), do)
+    want = ops.rel_attention_grad(ops.rel_attention_train(*(t.detach() for t in (q, k, v, table)), m)[1], do)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[3].dtype == torch.float32
+    same = torch.autograd.grad(ops.rel_attention(q, q, q, table, m), q, do)[0]                 # one tensor in three places
+    parts = ops.rel_attention_grad(ops.rel_attention_train(q.detach(), q.detach(), q.detach(), table.detach(), m)[1], do)[:3]
+    total = sum(t.double() for t in parts)
+    assert float((same.double() - total).norm()) <= 3 * R.half_step(dtype) * float(sum(t.double().abs() for t in parts).norm())
