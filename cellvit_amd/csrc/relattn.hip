@@ -11,9 +11,11 @@ namespace {
 // 4 waves, wave w owns rows [16 MQ w, 16 MQ (w + 1)) of the tile; BK keys a step, two LDS buffers: the loads of the next tile run behind the products of
 // this one, one barrier a tile.  Heads up to 64 wide: three waves a SIMD hide more than fragments read ahead (ragged training step: 561 us, 585 with
 // two waves and all fragments ahead); wider ones have registers for two waves at most.
-// 8 x 16 heads x 4096 x 80 fp16: 880 us, 780 TFLOP/s; bound by issue: a 16 x 16 block takes a SIMD 235 cycles, 88 of products (heads padded to 96 in the
-// first) and about 130 of VALU, half of that the exponentials; the two waves of a SIMD overlap them little.
-// REST (training): the sums of what rounding P left, too; a second set of accumulators leaves two waves a SIMD for heads up to 64 (the third would spill).
+// 8 x 16 heads x 4096 x 80 fp16: 880 to 900 us, 770 TFLOP/s; bound by issue: a 16 x 16 block takes a SIMD 232 cycles, 88 of products (heads padded to 96 in
+// the first) and 129 of VALU, half of that the exponentials; the two waves of a SIMD overlap them little.
+// REST (training): the sums of what rounding P left, too.  The parts cost VALU (three to four instructions an element in fp16, five in bf16) and products: 24 x 12 heads
+// x up to 1500 x 64 bf16 198 us, 114 without; causal 2 x 16 x 4096 x 128 fp16 260, 203.  The second set of accumulators leaves two waves a SIMD for heads up to
+// 64 (the third would spill: no gain).
 template <typename T, int DT, int MQ, int BK, bool REST>
 __global__ __launch_bounds__(256, DT > 64 || REST ? 2 : 3) void rel_attn_kernel(const RelAttn k) {
     typedef Dims<DT> Dm;
