@@ -379,6 +379,8 @@ def rel_attention_grad(saved: RelAttentionSaved, dout: torch.Tensor, *, table_gr
     _no_tangents(s.q, s.k, s.v, s.table, dout)
     if dout.shape != s.out.shape or dout.dtype != s.out.dtype:
         raise ValueError(f"dout must be {s.out.dtype} {list(s.out.shape)}")
+    if s.out_lo is not None and (s.out_lo.dtype is not _F32 or s.out_lo.shape != s.out.shape or not s.out_lo.is_contiguous()):
+        raise ValueError("saved.out_lo must be contiguous float32 of out's shape, as rel_attention_train returns it")
     c = _attn_setup(s.q, s.k, s.v, s.table, s.buckets, s.scale, s.causal, s.q_offsets, s.k_offsets, s.max_q, s.max_k, 1)
     _same_device(s.q, dout)
     dout, sd = _rows(dout, 16 // dout.element_size())

@@ -304,3 +304,38 @@ def test_autograd_with_a_float32_table_equals_the_halves(dtype):
     parts = ops.rel_attention_grad(ops.rel_attention_train(q.detach(), q.detach(), q.detach(), table.detach(), m)[1], do)[:3]
     total = sum(t.double() for t in parts)
     assert float((same.double() - total).norm()) <= 3 * R.half_step(dtype) * float(sum(t.double().abs() for t in parts).norm())
+
+
+@TYPES
+@pytest.mark.parametrize("lens", [(150, 170), (2, 900)])
+def test_the_c_entries_take_any_form_of_what_rounding_took(dtype, lens):
+    """out_lo in fp32, in the call's type, or none: the same output, and gradients as good as D allows."""
+    from cellvit_amd import _lib
+    lib, code = _lib.load(), {F16: _lib.DTYPE_F16, BF16: _lib.DTYPE_BF16, F32: _lib.DTYPE_F32}[dtype]
+    g = torch.Generator().manual_seed(40)
+    (lq, lk), H, D = lens, 2, 64
+    q, k, v, do = (torch.randn(n, H, D, generator=g).to(dtype) for n in (lq, lk, lk, lq))
+    table, m = torch.randn(32, H, generator=g), _map(32, 64, True)
+    dev = [t.cuda() for t in (q, k, v, do, table, m)]
+    ref = R.attention(q, k, v, table, m, 0.125, False, do)
+    off, outs = [], []
+    for lo in (torch.full((lq, H, D), 7.0, device="cuda"), torch.full((lq, H, D), 7.0, dtype=dtype, device="cuda"), None):
+        out, dq, dk, dv = (torch.empty(n, H, D, dtype=dtype, device="cuda") for n in (lq, lq, lk, lk))
+        lse, dt = torch.empty(lq, H, device="cuda"), torch.empty(32, H, device="cuda")
+        a = _lib.cv_rel_attn(dtype=code, n_seq=1, heads=H, kv_heads=H, head_dim=D, max_q=lq, max_k=lk, num_buckets=32, span=64, scale=0.125, table_dtype=_lib.DTYPE_F32,
+                             lo_f32=int(lo is not None and lo.dtype is F32), q_row=H * D, q_head=D, k_row=H * D, k_head=D, v_row=H * D, v_head=D, o_row=H * D, o_head=D, do_row=H * D, do_head=D,
+                             q=dev[0].data_ptr(), k=dev[1].data_ptr(), v=dev[2].data_ptr(), table=dev[4].data_ptr(), map=dev[5].data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
+                             out_lo=None if lo is None else lo.data_ptr(), dout=dev[3].data_ptr(), dq=dq.data_ptr(), dk=dk.data_ptr(), dv=dv.data_ptr(), dtable=dt.data_ptr())
+        for grad, fn in enumerate((lib.cv_op_rel_attention, lib.cv_op_rel_attention_grad)):
+            need = lib.cv_op_rel_attention_ws(C.byref(a), grad)
+            ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+            a.ws, a.ws_bytes = ws.data_ptr(), need
+            _lib.check(fn(C.byref(a), torch.cuda.current_stream().cuda_stream))
+            torch.cuda.synchronize()
+        for name, x in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv), ("dtable", dt)):
+            _close(x, *ref[name], name)
+        outs.append(out)
+        off.append(float((dt.double().cpu() - ref["dtable"][0]).norm() / ref["dtable"][0].norm()))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    if dtype != F32:                                                         # D good to fp32, to about 16 bits more than `dtype`, to `dtype`
+        assert off[0] <= 2.0 ** -17 and off[1] <= 2.0 ** -14 and off[0] <= off[2] and off[1] <= off[2]

@@ -89,3 +89,12 @@ def test_sizes_beyond_32_bits_are_refused_and_wide_gate_groups_are_one_group(mon
     for per in (6, 7, 1 << 31, 1 << 40):
         seqops.block_norm(x, x, gate=t(1, 32), rows_per_gate=per)
     assert len(calls) == 4 and len({a[:24] for a in calls}) == 1               # the head of the struct: sizes and rows a group
+
+
+def test_what_rounding_took_must_be_float32():
+    t = torch.zeros
+    q = t(1, 5, 2, 16).half()
+    saved = seqops.RelAttentionSaved(q, q, q, None, None, None, None, q, t(1, 5, 2), t(1, 5, 2, 16), 0.25, False, 5, 5)
+    for bad in (q, t(1, 5, 2, 8), t(1, 5, 16, 2).transpose(2, 3)):
+        with pytest.raises(ValueError, match="out_lo"):
+            seqops.rel_attention_grad(saved._replace(out_lo=bad), q)
