@@ -339,3 +339,18 @@ def test_the_c_entries_take_any_form_of_what_rounding_took(dtype, lens):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
     if dtype != F32:                                                         # D good to fp32, to about 16 bits more than `dtype`, to `dtype`
         assert off[0] <= 2.0 ** -17 and off[1] <= 2.0 ** -14 and off[0] <= off[2] and off[1] <= off[2]
+
+
+@TYPES
+@pytest.mark.parametrize("batch,heads,q,k", [(64, 2, 257, 257), (512, 1, 130, 131), (3, 2, 1000, 700)])
+def test_a_planes_gradient_summed_over_a_batch_of_one_sign(dtype, batch, heads, q, k):
+    """Values near 0.1: every addition to a running sum errs the same way.  A lane adds runs of 128 rows, the batch's runs with compensation (2^-23 in all), and the
+    diagonals and parts in trees of some 30 additions: (128 + 30) 2^-24 of the sum at the worst."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(43)
+    d = (0.1 + 0.001 * torch.rand(batch, heads, q, k, generator=g)).to(dtype)
+    m = _map(32, 128, True)
+    got = ops.rel_bias_grad(d.cuda(), m.cuda(), 32).double().cpu()
+    plane, total = R.bucket_plane(m, q, k).reshape(-1), d.double().sum(0).reshape(heads, -1)
+    want = torch.zeros(32, heads, dtype=torch.float64).index_add_(0, plane, total.T)
+    assert float(((got - want).abs() / want.abs().clamp(min=1e-30)).max()) <= 160 * 2.0 ** -24
