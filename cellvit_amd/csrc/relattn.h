@@ -246,7 +246,13 @@ int64_t rel_attention_bwd_tiles(const cv_rel_attn& a);
 int launch_rel_zero(void* base, int dtype, long rows, int heads, int D, long row, long head, hipStream_t st);
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
+// ref + log2(sum) rounded once: the sum's exponent is added exactly, so the logarithm that the hardware rounds is one of 1/2 .. 1.  (Of the whole sum it is off by
+// a step of 8 or more, towards below on average, and the backward's P of the row with it.)
+__device__ __forceinline__ float lse_of(float ref, float sum) {
+    const float e = (float)__builtin_amdgcn_frexp_expf(sum), s = ref + e, part = s - ref;
+    const float lost = (ref - (s - part)) + (e - part);
+    return s + (lost + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sum)));
+}
 // four or eight neighbouring results, rounded
 template <typename T, int N, typename V> __device__ __forceinline__ void store_rounded(T* dst, const V& x) {
     typedef T tn __attribute__((ext_vector_type(N)));

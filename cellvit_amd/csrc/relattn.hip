@@ -264,7 +264,7 @@ __global__ __launch_bounds__(256, DT > 64 || REST ? 2 : 3) void rel_attn_kernel(
             continue;
         }
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;    // an empty row: zeros; NaN stays NaN
-        if (a.lse && g4 == 0) a.lse[row] = sum > 0.f ? mref[m] + log2_hw(sum) : sum == 0.f ? NEG_INF : sum;
+        if (a.lse && g4 == 0) a.lse[row] = sum > 0.f ? lse_of(mref[m], sum) : sum == 0.f ? NEG_INF : sum;
         T* ob = reinterpret_cast<T*>(a.out) + (a.q_off ? (qr.row0 + qi) * a.o_row : s * a.o_seq + qi * a.o_row) + h * a.o_head;
 #pragma unroll
         for (int d = 0; d < Dm::ND; ++d) {
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DT > 96 ? 1 : 2) void rel_at
     const float inv = tot > 0.f ? 1.f / tot : tot == 0.f ? 0.f : tot;
     if ((threadIdx.x & 15) == 0) {
         if (k.nsplit > 1) { k.part_ml[pr * 2] = ref; k.part_ml[pr * 2 + 1] = tot; }
-        else if (a.lse) a.lse[out_row] = tot > 0.f ? ref + log2_hw(tot) : tot == 0.f ? NEG_INF : tot;
+        else if (a.lse) a.lse[out_row] = tot > 0.f ? lse_of(ref, tot) : tot == 0.f ? NEG_INF : tot;
     }
     T* ob = reinterpret_cast<T*>(a.out) + (a.q_off ? (qr.row0 + qrow) * a.o_row : s * a.o_seq + qrow * a.o_row) + h * a.o_head;
     for (int c = (threadIdx.x & 15) * 4; c < D; c += 64) {
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(256) void rel_attn_join_kernel(const RelAttn k) {
         if constexpr (REST) left[j] = sum_over_groups(left[j]);
     }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-    if (a.lse && lane == 0) a.lse[(qr.row0 + qi) * a.heads + h] = l > 0.f ? ref + log2_hw(l) : l == 0.f ? NEG_INF : l;
+    if (a.lse && lane == 0) a.lse[(qr.row0 + qi) * a.heads + h] = l > 0.f ? lse_of(ref, l) : l == 0.f ? NEG_INF : l;
     if (lane >= 16 || c >= D) return;
     T* ob = reinterpret_cast<T*>(a.out) + (a.q_off ? (qr.row0 + qi) * a.o_row : s * a.o_seq + qi * a.o_row) + h * a.o_head + c;
 #pragma unroll

@@ -354,3 +354,15 @@ def test_a_planes_gradient_summed_over_a_batch_of_one_sign(dtype, batch, heads, 
     plane, total = R.bucket_plane(m, q, k).reshape(-1), d.double().sum(0).reshape(heads, -1)
     want = torch.zeros(32, heads, dtype=torch.float64).index_add_(0, plane, total.T)
     assert float(((got - want).abs() / want.abs().clamp(min=1e-30)).max()) <= 160 * 2.0 ** -24
+
+
+@TYPES
+def test_logarithms_of_the_sums_err_to_both_sides(dtype):
+    """lse is near 8 .. 12, where a step is 2^-20: rounded once, to both sides alike; the logarithm of 1/2 .. 1 and the exponentials may lean by a step of 2^-24 each."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(44)
+    q, k = (torch.randn(1, 1500, 2, 64, generator=g).to(dtype) for _ in range(2))
+    lse = ops.rel_attention_train(q.cuda(), k.cuda(), k.cuda())[1].lse.double().cpu()[0]
+    s = q[0].double().transpose(0, 1) @ k[0].double().permute(1, 2, 0) * 0.125
+    off = lse - torch.logsumexp(s, 2).T / math.log(2)
+    assert float(off.abs().max()) <= 2.0 ** -19 and abs(float(off.mean())) <= 2.0 ** -23
