@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, DT > 64 || REST ? 2 : 3) void rel_attn_kernel(
                 for (int d = 0; d < Dm::ND; ++d) {
                     const v8<T> v = u < VA ? vf[u < VA ? u : 0][d] : frag_col(vt, PT, u * 32, d * 16, g4, li);
 #pragma unroll
-                    for (int m = 0; m < MQ; ++m) o[m][d] = Seq<T>::mma(v, pf[m], o[m][d]);
+                    for (int m = 0; m < MQ; ++m) o[m][d] = mma_sum<T>(v, pf[m], o[m][d]);
                     if constexpr (REST) {
 #pragma unroll
                         for (int x = 0; x < Rest<T>::PARTS; ++x)
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DT > 96 ? 1 : 2) void rel_at
 #pragma unroll
         for (int d = 0; d < Dm::ND; ++d) {
             const v8<T> v = frag_col(vt, PT, 0, d * 16, g4, li);
-            o[d] = Seq<T>::mma(v, pf, o[d]);
+            o[d] = mma_sum<T>(v, pf, o[d]);
             if constexpr (REST) {
 #pragma unroll
                 for (int x = 0; x < Rest<T>::PARTS; ++x) rest[d] = Seq<T>::mma(v, rf[x], rest[d]);

@@ -367,7 +367,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DT <= 64 ? 4 : DT <= 96 ? 3 
                 if constexpr (SCALED<T>) { sc[2 * u] *= up; sc[2 * u + 1] *= up; }
                 const v8<T> pf = frag_acc<T>(sc[2 * u], sc[2 * u + 1]);      // dS rounded to T once, for the product only
 #pragma unroll
-                for (int d = 0; d < Dm::ND; ++d) o[d] = Seq<T>::mma(kc[u][d], pf, o[d]);
+                for (int d = 0; d < Dm::ND; ++d) o[d] = mma_sum<T>(kc[u][d], pf, o[d]);
             }
         }
         if (next < kend) {
@@ -671,8 +671,8 @@ __global__ __launch_bounds__(256, grad_waves<T>(DT)) void rel_attn_dkv_kernel(co
                 for (int d = 0; d < Dm::ND; ++d)
 #pragma unroll
                     for (int m = 0; m < MK; ++m) {
-                        dv[m][d] = Seq<T>::mma(dc[u][d], pf[u][m], dv[m][d]);
-                        dk[m][d] = Seq<T>::mma(qc[u][d], sf[u][m], dk[m][d]);
+                        dv[m][d] = mma_sum<T>(dc[u][d], pf[u][m], dv[m][d]);
+                        dk[m][d] = mma_sum<T>(qc[u][d], sf[u][m], dk[m][d]);
                     }
         });
     } else if (role == 0) {
