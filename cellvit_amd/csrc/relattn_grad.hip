@@ -70,8 +70,9 @@ template <int CTRL> __device__ __forceinline__ float dpp_shift(float v) {
 // its lower end, diagonals 4 g4 + 1 .. 3, is lanes 13 .. 15 of the next block of keys, where it is carried to.  So a lane's sum of a block belongs to one
 // offset, 16 further a block, and to one bucket for many blocks: it stays in a register until some lane's bucket changes.  Where one bucket ends, its
 // lanes' sums are added over the wave; where several do (near the diagonal) the wave's sums are put in the order of their offsets through LDS
-// and added by bucket.  (Causal step of 2 x 16 heads x 4096 x 128, right after a pause: 486 us, 446 with the case of one bucket by itself, 363 without table; 400 in a run of steps.  Adding
-// every block's sums to LDS by atomics cost 100 cycles an instruction, 60 % of the kernel.)  A tile beyond the span adds to one sum a lane.
+// and added by bucket.  (Causal step of 2 x 16 heads x 4096 x 128, right after a pause: 486 us, 446 with the case of one bucket by itself, 363 without table;
+// 400 in a run of steps.  Adding every block's sums to LDS by atomics cost 100 cycles an instruction, 60 % of the kernel.)  A tile beyond the span adds to
+// one sum a lane.
 // Bound by issue: of 24 products' 384 cycles a tile and wave a third runs at once with the loads, exponentials and sums of the other waves.
 // Closer to the diagonal than ZONE the sums are kept by offset, and added by bucket at the end: buckets are narrow there (ragged step of 24 x 12 heads x
 // 64, span 128: 518 us without, 506; 516 with 48 or 240, whose LDS and last sums cost what they save).
